@@ -33,7 +33,9 @@ extern "C" {
 typedef struct srx_context* srx_handle_t;
 typedef struct srx_mfcc_plan* srx_mfcc_plan_t;
 
-enum srx_dtype { SRX_F32 = 0, SRX_F64 = 1 };
+/* SRX_BF16 and SRX_F16 are element types of the trainable frame operators (the end of this
+ * file) only, which in turn have no SRX_F64 form. */
+enum srx_dtype { SRX_F32 = 0, SRX_F64 = 1, SRX_BF16 = 2, SRX_F16 = 3 };
 
 enum srx_status {
     SRX_OK = 0,
@@ -348,6 +350,135 @@ int srx_column_moments(srx_handle_t h, const void* X, int dtype, int64_t n_frame
  * applied in place to every model of the bank from its statistics record. */
 int srx_mstep(srx_handle_t h, const double* stats, const srx_priors_t* priors, int mode,
               const srx_models_t* models, void* stream);
+
+/* ---- trainable frame operators: the layers of an acoustic model that is trained by gradients
+ * and stands in front of the decoder in place of the Gaussians (its log-densities go to
+ * srx_viterbi_dense, its targets come from srx_posteriors).  The reference has none of them.
+ * Frames are packed by utterance as everywhere in this file.  Differences to the entry points
+ * above:
+ *   - element types SRX_F32, SRX_BF16, SRX_F16; parameters, states of the scan, statistics and the
+ *     gradients of parameters are float (32 bits) whatever the element type, all arithmetic is in 32
+ *     bits, and a result is rounded to the element type once;
+ *   - matrices of frames have a row pitch in elements (`ld_*`, at least the row's width), so that
+ *     parts of a wider projection are taken as they are; nothing needs more than its element's alignment;
+ *   - scratch is the caller's (`workspace`, sized by the *_workspace functions; NULL where that is 0):
+ *     nothing is allocated, so the calls may be captured into graphs, and calls with
+ *     workspaces of their own may run at the same time on several streams;
+ *   - the caller's current device is left as it was;
+ *   - frames before utt_offsets[0] and from utt_offsets[n_utts] on belong to no utterance: their
+ *     rows in every output are left as they were. */
+
+/* Short causal convolution over the frames of each channel, one filter per channel:
+ *   y[t, c] = act(bias[c] + sum_k weight[c, k] x[t - width + 1 + k, c])
+ * The width - 1 frames before an utterance are those of state_in[n_utts, width - 1, n_channels]
+ * (element type, oldest first), zeros without it; state_out (may be state_in) receives the last width - 1
+ * frames, those of state_in among them where the utterance is shorter.  The delta regression of the
+ * front-end (mfcc.py:82-96) is the fixed, centred relative of it. */
+enum srx_activation { SRX_IDENTITY = 0, SRX_SILU = 1 };
+typedef struct {
+    int32_t n_channels;
+    int32_t width;          /* 1 .. 8 */
+    int32_t activation;
+    int32_t reserved;
+    const float* weight;    /* [n_channels, width] */
+    const float* bias;      /* [n_channels] or NULL */
+} srx_conv_t;
+int srx_causal_conv(srx_handle_t h, const srx_conv_t* conv, int dtype, const void* x, int64_t ld_x,
+                    const int64_t* utt_offsets, int64_t n_utts, int64_t n_frames, const void* state_in,
+                    void* state_out, void* y, int64_t ld_y, void* stream);
+/* One frame of each of n_rows streams: y from state[n_rows, width - 1, n_channels] and x, the
+ * state moved on by the frame, in place. */
+int srx_causal_conv_step(srx_handle_t h, const srx_conv_t* conv, int dtype, const void* x, int64_t ld_x,
+                         int64_t n_rows, void* state, void* y, int64_t ld_y, void* stream);
+/* Gradients of srx_causal_conv: dx (element type) and dweight[n_channels, width], dbias[n_channels] (or NULL);
+ * with state_in also dstate_in[n_utts, width - 1, n_channels] (element type, may be NULL); dstate_out
+ * (element type, or NULL for zeros) is the gradient that comes in for state_out. */
+int64_t srx_causal_conv_backward_workspace(srx_handle_t h, const srx_conv_t* conv, int64_t n_utts, int64_t n_frames);
+int srx_causal_conv_backward(srx_handle_t h, const srx_conv_t* conv, int dtype, const void* x, int64_t ld_x,
+                             const int64_t* utt_offsets, int64_t n_utts, int64_t n_frames, const void* state_in,
+                             const void* dy, int64_t ld_dy, const void* dstate_out, void* dx, int64_t ld_dx,
+                             float* dweight, float* dbias, void* dstate_in, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* Selective state space scan: a linear recurrence per channel and state whose decay, input and
+ * output weights depend on the frame,
+ *   d = softplus(dt[t, c] + dt_bias[c])        (dt[t, c] + dt_bias[c] without softplus)
+ *   h[t, c, n] = exp(d A[c, n]) h[t-1, c, n] + d x[t, c] B[t, g(c), n]
+ *   y[t, c] = (sum_n C[t, g(c), n] h[t, c, n] + skip[c] x[t, c]) silu(gate[t, c])
+ * -- the recursion of srx_forward_score's alpha with a diagonal, frame-dependent transition and no
+ * normalisation.  g(c) = c / (n_channels / n_groups): neighbouring channels share B and C.  h starts from
+ * state_in[n_utts, n_channels, n_states] (zeros if NULL); state_out (may be state_in, may be NULL) receives
+ * the states behind the last frames, those of state_in for an utterance without frames. */
+typedef struct {
+    int32_t n_channels;
+    int32_t n_states;       /* 1 .. 64 */
+    int32_t n_groups;       /* a divisor of n_channels */
+    int32_t softplus;       /* 0 / 1 */
+    const float* A;         /* [n_channels, n_states] */
+    const float* skip;      /* [n_channels] or NULL */
+    const float* dt_bias;   /* [n_channels] or NULL */
+} srx_scan_t;
+/* Inputs of the scan, one row per frame: n_channels values of x, dt and gate (NULL: no gate), n_groups x
+ * n_states of B and C. */
+typedef struct {
+    const void *x, *dt, *B, *C, *gate;
+    int64_t ld_x, ld_dt, ld_B, ld_C, ld_gate;
+} srx_scan_inputs_t;
+/* Where the gradients of the inputs go (dgate: NULL without a gate), the same way. */
+typedef struct {
+    void *dx, *ddt, *dB, *dC, *dgate;
+    int64_t ld_dx, ld_ddt, ld_dB, ld_dC, ld_dgate;
+} srx_scan_gradients_t;
+/* Floats of `saved`: states that a training pass keeps for srx_selective_scan_backward (every eighth frame's). */
+int64_t srx_selective_scan_saved(const srx_scan_t* scan, int64_t n_utts, int64_t n_frames);
+int64_t srx_selective_scan_workspace(srx_handle_t h, const srx_scan_t* scan, int64_t n_utts, int64_t n_frames);
+/* saved: NULL, or srx_selective_scan_saved floats to fill. */
+int srx_selective_scan(srx_handle_t h, const srx_scan_t* scan, const srx_scan_inputs_t* in, int dtype,
+                       const int64_t* utt_offsets, int64_t n_utts, int64_t n_frames, const float* state_in,
+                       float* state_out, void* y, int64_t ld_y, float* saved, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+/* One frame of each of n_rows streams, state[n_rows, n_channels, n_states] moved on in place. */
+int srx_selective_scan_step(srx_handle_t h, const srx_scan_t* scan, const srx_scan_inputs_t* in, int dtype,
+                            int64_t n_rows, float* state, void* y, int64_t ld_y, void* stream);
+/* Gradients of srx_selective_scan from dy and what its pass over the same inputs saved: those of the inputs in
+ * `grads`, dA[n_channels, n_states], dskip and dt_bias' [n_channels] (NULL where the parameter is), and
+ * dstate_in (NULL if not wanted); dstate_out: the gradient that comes in for state_out, NULL for zeros.
+ * Sums over frames and channels are taken in a fixed order: the same inputs give the same bits. */
+int64_t srx_selective_scan_backward_workspace(srx_handle_t h, const srx_scan_t* scan, int64_t n_utts,
+                                              int64_t n_frames);
+int srx_selective_scan_backward(srx_handle_t h, const srx_scan_t* scan, const srx_scan_inputs_t* in, int dtype,
+                                const int64_t* utt_offsets, int64_t n_utts, int64_t n_frames,
+                                const float* saved, const void* dy, int64_t ld_dy, const float* dstate_out,
+                                const srx_scan_gradients_t* grads, float* dA, float* dskip, float* ddt_bias,
+                                float* dstate_in, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Layer norm of every row: y = (x - mean) rstd weight + bias with the row's own mean and rstd =
+ * 1 / sqrt(variance + eps) (variance over n, not n - 1), which are returned (mean, rstd: n_rows floats).
+ * weight, bias: n_features floats, or NULL for ones and zeros.  The z-score of the front-end
+ * (HMM_final.py:18-23) is the same along the other axis. */
+int srx_layer_norm(srx_handle_t h, const void* x, int64_t ld_x, int dtype, int64_t n_rows, int32_t n_features,
+                   const float* weight, const float* bias, double eps, void* y, int64_t ld_y, float* mean,
+                   float* rstd, void* stream);
+int64_t srx_layer_norm_backward_workspace(srx_handle_t h, int64_t n_rows, int32_t n_features);
+/* dx, and dweight, dbias (n_features floats, NULL if not wanted) from dy, x and the mean and rstd of the
+ * forward pass; sums over the rows in a fixed order. */
+int srx_layer_norm_backward(srx_handle_t h, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int dtype,
+                            int64_t n_rows, int32_t n_features, const float* mean, const float* rstd,
+                            const float* weight, void* dx, int64_t ld_dx, float* dweight, float* dbias,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradient clipping: out_norm[0] = the root of the sum of squares over all values of n_tensors tensors
+ * (accumulated in 64 bits), and every tensor times min(1, max_norm / (norm + 1e-6)), the factor in 32
+ * bits.  Host arrays: tensors[n_tensors] device pointers, counts their numbers of values (0 allowed),
+ * dtypes theirs; outs NULL for in place, else device pointers of tensors that receive the product, out_dtypes
+ * (the tensor's own type, or SRX_F32).  In place the values are not touched where the factor is
+ * 1; a norm that is not finite leaves the values as they are (outs: a copy) and says so by itself.
+ * Tensors that are written may not overlap one another, nor other tensors (SRX_EINVAL).  The arrays are read
+ * before the call returns. */
+int64_t srx_clip_gradients_workspace(srx_handle_t h, int64_t n_tensors, const int64_t* counts);
+int srx_clip_gradients(srx_handle_t h, int64_t n_tensors, void* const* tensors, const int64_t* counts,
+                       const int32_t* dtypes, void* const* outs, const int32_t* out_dtypes, double max_norm,
+                       double* out_norm, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

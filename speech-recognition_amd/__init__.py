@@ -9,10 +9,12 @@ All arithmetic runs in libsrx.so (hand-written HIP for gfx950, C ABI in
 include/srx.h); importing the package fails if that library is not built.
 """
 from . import _lib                      # noqa: F401  (raises if libsrx.so is missing)
-from . import runtime, hmm, mfcc, endpoint, recognizer, hmm_lib, parallel, SpeechUtil   # noqa: F401
+from . import runtime, hmm, mfcc, endpoint, recognizer, hmm_lib, parallel, ssm, SpeechUtil   # noqa: F401
 from .hmm import MyGaussianHMM, GaussianHMM, ConvergenceMonitor        # noqa: F401
 from .runtime import (Context, HMMBank, Ragged, MfccPlan, GmmEmission, viterbi_dense,   # noqa: F401
                       argmax_scores, column_moments)
+from .ssm import (selective_scan, selective_scan_backward, selective_scan_step, causal_conv,   # noqa: F401
+                  causal_conv_backward, causal_conv_step, layer_norm, layer_norm_backward, clip_gradients)
 
 HMM_final = recognizer   # the reference's module name for the same functions
 HMM_lib = hmm_lib         # likewise (librosa-convention features, hmmlearn-style models)

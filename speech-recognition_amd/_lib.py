@@ -14,7 +14,8 @@ import torch  # noqa: F401
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SRX_LIB") or os.path.join(_HERE, "libsrx.so")
 
-SRX_F32, SRX_F64 = 0, 1
+SRX_F32, SRX_F64, SRX_BF16, SRX_F16 = 0, 1, 2, 3
+SRX_IDENTITY, SRX_SILU = 0, 1
 SRX_MSTEP_FULL, SRX_MSTEP_TRANSITIONS_ONLY = 0, 1
 SRX_OPT_EXACT_F32 = 1
 SRX_OPT_ESTEP_PATH = 2
@@ -61,6 +62,26 @@ class EndpointCfg(C.Structure):
                 ("reserved", C.c_int32), ("noise_peak", C.c_double)]
 
 
+class Conv(C.Structure):
+    _fields_ = [("n_channels", C.c_int32), ("width", C.c_int32), ("activation", C.c_int32),
+                ("reserved", C.c_int32), ("weight", C.c_void_p), ("bias", C.c_void_p)]
+
+
+class Scan(C.Structure):
+    _fields_ = [("n_channels", C.c_int32), ("n_states", C.c_int32), ("n_groups", C.c_int32),
+                ("softplus", C.c_int32), ("A", C.c_void_p), ("skip", C.c_void_p), ("dt_bias", C.c_void_p)]
+
+
+class ScanInputs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "dt", "B", "C", "gate")] + \
+               [("ld_" + n, C.c_int64) for n in ("x", "dt", "B", "C", "gate")]
+
+
+class ScanGradients(C.Structure):
+    _fields_ = [("d" + n, C.c_void_p) for n in ("x", "dt", "B", "C", "gate")] + \
+               [("ld_d" + n, C.c_int64) for n in ("x", "dt", "B", "C", "gate")]
+
+
 _vp, _i64, _i32 = C.c_void_p, C.c_int64, C.c_int32
 
 # name -> (restype, argtypes); must list every symbol include/srx.h declares.
@@ -96,6 +117,27 @@ SIGNATURES = {
     "srx_mstep": (C.c_int, [_vp, _vp, C.POINTER(Priors), C.c_int, C.POINTER(Models), _vp]),
     "srx_gmm_emission_loglik": (C.c_int, [_vp, _vp, C.c_int, _i64, C.POINTER(Gmm), _vp, _vp]),
     "srx_posteriors": (C.c_int, [_vp, _vp, C.c_int, _vp, _i64, _i64, _vp, C.POINTER(Models), _vp, _vp, _vp]),
+    "srx_causal_conv": (C.c_int, [_vp, C.POINTER(Conv), C.c_int, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
+    "srx_causal_conv_step": (C.c_int, [_vp, C.POINTER(Conv), C.c_int, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "srx_causal_conv_backward_workspace": (_i64, [_vp, C.POINTER(Conv), _i64, _i64]),
+    "srx_causal_conv_backward": (C.c_int, [_vp, C.POINTER(Conv), C.c_int, _vp, _i64, _vp, _i64, _i64, _vp, _vp,
+                                           _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "srx_selective_scan_saved": (_i64, [C.POINTER(Scan), _i64, _i64]),
+    "srx_selective_scan_workspace": (_i64, [_vp, C.POINTER(Scan), _i64, _i64]),
+    "srx_selective_scan": (C.c_int, [_vp, C.POINTER(Scan), C.POINTER(ScanInputs), C.c_int, _vp, _i64, _i64, _vp,
+                                     _vp, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "srx_selective_scan_step": (C.c_int, [_vp, C.POINTER(Scan), C.POINTER(ScanInputs), C.c_int, _i64, _vp, _vp,
+                                          _i64, _vp]),
+    "srx_selective_scan_backward_workspace": (_i64, [_vp, C.POINTER(Scan), _i64, _i64]),
+    "srx_selective_scan_backward": (C.c_int, [_vp, C.POINTER(Scan), C.POINTER(ScanInputs), C.c_int, _vp, _i64, _i64,
+                                              _vp, _vp, _i64, _vp, C.POINTER(ScanGradients), _vp, _vp, _vp, _vp,
+                                              _vp, _i64, _vp]),
+    "srx_layer_norm": (C.c_int, [_vp, _vp, _i64, C.c_int, _i64, _i32, _vp, _vp, C.c_double, _vp, _i64, _vp, _vp, _vp]),
+    "srx_layer_norm_backward_workspace": (_i64, [_vp, _i64, _i32]),
+    "srx_layer_norm_backward": (C.c_int, [_vp, _vp, _i64, _vp, _i64, C.c_int, _i64, _i32, _vp, _vp, _vp, _vp, _i64,
+                                          _vp, _vp, _vp, _i64, _vp]),
+    "srx_clip_gradients_workspace": (_i64, [_vp, _i64, _vp]),
+    "srx_clip_gradients": (C.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, C.c_double, _vp, _vp, _i64, _vp]),
     "srx_viterbi_dense": (C.c_int, [_vp, _vp, C.c_int, _vp, _i64, _i64, C.c_int32, _vp, _vp, _vp, _vp, _vp]),
 }
 

@@ -21,6 +21,12 @@ FILE_FLAGS = {"score_mfma.hip": ["-fno-slp-vectorize"], "score_split8.hip": ["-f
               # vectoriser it needs a move per pair and runs 7 % slower)
               "mfcc_fast.hip": ["-fno-slp-vectorize"],
               "mfcc_wide.hip": ["-fno-slp-vectorize"]}
+# The trainable frame operators have no packed f32 instructions at all: neither the vectoriser's
+# nor the instruction selection's (the host pass warns that it does not know the feature).
+FRAME_SOURCES = ["ssm_scan.hip", "ssm_scan_f32.hip", "ssm_scan_bf16.hip", "ssm_scan_f16.hip", "ssm_conv.hip",
+                 "layer_norm.hip", "grad_clip.hip"]
+FILE_FLAGS.update({s: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for s in FRAME_SOURCES})
+SOURCES += FRAME_SOURCES
 FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Wall",
          "-Wno-unused-function", "-fvisibility=default",
          "-I", os.path.join(ROOT, "include"), "-I", CSRC]

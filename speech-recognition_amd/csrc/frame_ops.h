@@ -1,0 +1,140 @@
+// What the trainable frame operators (selective scan, short convolution, layer norm, gradient
+// clipping) share: element types of two and four bytes, vector loads and stores that need no more
+// than the element's own alignment, sums over parts of a wave, and the guard that leaves the
+// caller's current device as it was.
+#pragma once
+#include "srx_internal.h"
+
+#include <string.h>
+
+namespace srx_frames {
+
+template <typename T, int V>
+struct Pack {
+    T v[V];
+};
+
+// V neighbouring elements as one memory instruction: gfx950 takes global accesses at any
+// alignment, and full width where the address happens to be aligned.
+template <int V, typename T>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+    Pack<T, V> r;
+    __builtin_memcpy(&r, (const void*)p, sizeof(r));
+    return r;
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
+    __builtin_memcpy((void*)p, &v, sizeof(v));
+}
+// The first `n` (<= V) of V neighbouring elements, zeros behind them.
+template <int V, typename T>
+__device__ __forceinline__ Pack<T, V> load_some(const T* p, int n) {
+    if (n >= V) return load_pack<V>(p);
+    Pack<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = i < n ? p[i] : (T)0.0f;
+    return r;
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_some(T* p, const Pack<T, V>& v, int n) {
+    if (n >= V) {
+        store_pack(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i < n) p[i] = v.v[i];
+}
+
+// e^x by the hardware's 2^x; the part of x log2(e) that its rounding to 32 bits drops is put
+// back to first order, so that the relative error does not grow with |x|.
+__device__ __forceinline__ float exp_f32(float x) {
+    const float kLog2e = 1.44269504088896341f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147180559945309f;
+    const float t = x * kLog2e;
+    const float rest = fmaf(x, kLog2e, -t) + x * kLog2eRest;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, rest * kLn2, e);
+}
+__device__ __forceinline__ float sigmoid_f32(float x) {
+    // (the exponential overflows to infinity for x below -88, the quotient is then zero)
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x));
+}
+// ln(1 + e^x) = max(x, 0) + log1p(e^-|x|); log1p(e) = 2 artanh(e / (2 + e)) by its power series,
+// whose argument is at most 1/3: seven terms leave 1.5e-8 of the value, and small values keep
+// their relative accuracy (steps of 0.001 and less are ordinary).
+__device__ __forceinline__ float softplus_f32(float x) {
+    const float e = exp_f32(-fabsf(x));
+    const float s = e * __builtin_amdgcn_rcpf(2.0f + e);
+    const float q = s * s;
+    float p = fmaf(q, 1.0f / 13.0f, 1.0f / 11.0f);
+    p = fmaf(p, q, 1.0f / 9.0f);
+    p = fmaf(p, q, 1.0f / 7.0f);
+    p = fmaf(p, q, 1.0f / 5.0f);
+    p = fmaf(p, q, 1.0f / 3.0f);
+    p = fmaf(p * q, 2.0f * s, 2.0f * s);
+    // (not fmaxf: a NaN has to come through)
+    return (x > 0.0f ? x : (x == x ? 0.0f : x)) + p;
+}
+
+// Orders the LDS traffic of one wave: its lanes read what other lanes of it wrote.  The hardware
+// runs a wave's LDS instructions in order; this keeps the compiler from moving them.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// a and b with their 32-lane halves (16-lane odd / even rows) exchanged and added: lanes of the
+// lower half (even rows) get the sum of a over the pair of lanes, the others that of b.
+__device__ __forceinline__ float halves_sum(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float rows_sum(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_mov(float v) {
+    const int i = __float_as_int(v);
+    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
+}
+// Sum over the 16 lanes of a row, in all of them.
+__device__ __forceinline__ float row16_sum(float v) {
+    v += dpp_mov<0x128>(v);     // row_ror:8
+    v += dpp_mov<0x124>(v);     // row_ror:4
+    v += dpp_mov<0x122>(v);     // row_ror:2
+    v += dpp_mov<0x121>(v);     // row_ror:1
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v = row16_sum(v);
+    v = rows_sum(v, v);
+    return halves_sum(v, v);
+}
+
+// Entry points run on the context's device and leave the caller's current device alone.
+struct DeviceGuard {
+    int before = -1, rc = SRX_OK;
+    explicit DeviceGuard(int device) {
+        rc = enter(device);
+    }
+    int enter(int device) {
+        int now = -1;
+        SRX_HIP(hipGetDevice(&now));
+        if (now != device) {
+            SRX_HIP(hipSetDevice(device));
+            before = now;
+        }
+        return SRX_OK;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    DeviceGuard(const DeviceGuard&) = delete;
+    DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
+
+inline bool frame_dtype(int dtype) { return dtype == SRX_F32 || dtype == SRX_BF16 || dtype == SRX_F16; }
+
+}  // namespace srx_frames

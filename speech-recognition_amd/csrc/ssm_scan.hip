@@ -1,0 +1,252 @@
+// Entry points of the selective state space scan: argument checks, the choice between whole
+// utterances and pieces of them, and the division of the caller's workspace (kernels: ssm_scan.h).
+#include "ssm_scan.h"
+
+namespace {
+
+// Channels of a wave's block: 16 R, by the number of states (see scan_dispatch).
+int block_channels(int states) { return states <= 16 ? 64 : states <= 32 ? 32 : 16; }
+int block_states(int states) { return states <= 4 ? 4 : states <= 8 ? 8 : states <= 16 ? 16 : states <= 32 ? 32 : 64; }
+
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+int check_scan(srx_handle_t h, const srx_scan_t* s, int64_t utts, int64_t frames, const char* who) {
+    SRX_REQUIRE(h != nullptr, "%s: NULL context", who);
+    SRX_REQUIRE(s != nullptr, "%s: scan is NULL", who);
+    SRX_REQUIRE(s->n_channels >= 1 && s->n_groups >= 1 && s->n_channels % s->n_groups == 0,
+                "%s: Shape mismatch (n_channels=%d n_groups=%d)", who, s->n_channels, s->n_groups);
+    SRX_REQUIRE(s->n_states >= 1 && s->n_states <= 64, "%s: n_states %d outside [1, 64]", who, s->n_states);
+    SRX_REQUIRE(s->A != nullptr, "%s: NULL A", who);
+    SRX_REQUIRE(utts >= 0 && frames >= 0, "%s: negative size", who);
+    return SRX_OK;
+}
+
+int check_inputs(const srx_scan_t* s, const srx_scan_inputs_t* in, int dtype, int64_t frames, const char* who) {
+    SRX_REQUIRE(frame_dtype(dtype), "%s: unknown dtype %d", who, dtype);
+    SRX_REQUIRE(in != nullptr, "%s: inputs are NULL", who);
+    if (frames == 0) return SRX_OK;
+    const int64_t c = s->n_channels, bc = (int64_t)s->n_groups * s->n_states;
+    SRX_REQUIRE(in->x && in->dt && in->B && in->C, "%s: NULL input", who);
+    SRX_REQUIRE(in->ld_x >= c && in->ld_dt >= c && in->ld_B >= bc && in->ld_C >= bc &&
+                    (in->gate == nullptr || in->ld_gate >= c),
+                "%s: a row pitch is smaller than its row", who);
+    return SRX_OK;
+}
+
+// The smallest pitches that a caller may pass keep every offset far below 2^63.
+ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, int64_t frames) {
+    ScanParams p;
+    memset(&p, 0, sizeof(p));
+    p.A = s->A;
+    p.skip = s->skip;
+    p.bias = s->dt_bias;
+    p.softplus = s->softplus;
+    p.channels = s->n_channels;
+    p.states = s->n_states;
+    p.groups = s->n_groups;
+    p.per_group = s->n_channels / s->n_groups;
+    const int ch = block_channels(s->n_states);
+    p.group_blocks = (p.per_group + ch - 1) / ch;
+    p.blocks = p.group_blocks * s->n_groups;
+    p.utts = utts;
+    p.frames = frames;
+    // Whole utterances where they alone give every SIMD two waves (a SIMD with a single wave issues at
+    // half its rate); else pieces, whose states are computed twice.
+    const int64_t wanted = (int64_t)h->n_cu * 4 * 2;
+    p.segment = 0;
+    p.units = utts;
+    if (utts > 0 && utts * p.blocks < wanted) {
+        const int64_t segment = round_up(frames * p.blocks / (2 * wanted) > 64 ? frames * p.blocks / (2 * wanted) : 64, 16);
+        if (frames / utts > 2 * segment) {
+            p.segment = segment;
+            p.units = frames / segment + utts;
+        }
+    }
+    // backward: a wave sums the parameters' gradients over all its units
+    p.parts = p.units;
+    const int64_t most = 4 * wanted / p.blocks + 1;
+    if (p.segment == 0 && p.parts > most) p.parts = most;
+    if (p.parts < 1) p.parts = 1;
+    return p;
+}
+
+// Hands out the workspace; with a NULL base it only counts.
+struct Carver {
+    char* base;
+    int64_t used = 0;
+    float* floats(int64_t n) {
+        float* at = base != nullptr ? (float*)(base + used) : nullptr;
+        used += round_up(n * 4, 256);
+        return at;
+    }
+};
+
+int64_t carve(ScanParams& p, bool backward, void* workspace) {
+    Carver c{(char*)workspace};
+    const int64_t ch = block_channels(p.states), ns = block_states(p.states);
+    if (p.segment != 0) {
+        p.seg_state = c.floats(p.units * p.blocks * ch * ns);
+        p.seg_sum = c.floats(p.units * p.blocks * ch);
+    }
+    if (backward) {
+        p.part_A = c.floats(p.parts * p.blocks * ch * ns);
+        p.part_vec = c.floats(p.parts * p.blocks * 2 * ch);
+        p.part_bc = c.floats(p.blocks * p.frames * 2 * ns);
+    }
+    return c.used;
+}
+
+int run(const ScanParams& p, int dtype, bool backward, hipStream_t st) {
+    switch (dtype) {
+        case SRX_F32: return scan_run<float>(p, backward, st);
+        case SRX_BF16: return scan_run<__bf16>(p, backward, st);
+        default: return scan_run<_Float16>(p, backward, st);
+    }
+}
+
+void take_inputs(ScanParams& p, const srx_scan_inputs_t* in) {
+    p.x = in->x;
+    p.dt = in->dt;
+    p.B = in->B;
+    p.C = in->C;
+    p.gate = in->gate;
+    p.ld_x = in->ld_x;
+    p.ld_dt = in->ld_dt;
+    p.ld_B = in->ld_B;
+    p.ld_C = in->ld_C;
+    p.ld_gate = in->ld_gate;
+}
+
+int64_t workspace_bytes_for(srx_handle_t h, const srx_scan_t* s, int64_t utts, int64_t frames, bool backward,
+                            const char* who) {
+    if (check_scan(h, s, utts, frames, who)) return -1;
+    ScanParams p = params_for(h, s, utts, frames);
+    return carve(p, backward, nullptr);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t srx_selective_scan_saved(const srx_scan_t* s, int64_t n_utts, int64_t n_frames) {
+    if (s == nullptr || s->n_channels < 1 || s->n_groups < 1 || s->n_states < 1 || s->n_states > 64 ||
+        s->n_channels % s->n_groups != 0 || n_utts < 0 || n_frames < 0) {
+        srx_set_error("srx_selective_scan_saved: Shape mismatch");
+        return -1;
+    }
+    const int64_t ch = block_channels(s->n_states), per = s->n_channels / s->n_groups;
+    return (n_frames / kScanSaveEvery + n_utts) * ((per + ch - 1) / ch * s->n_groups) * ch * block_states(s->n_states);
+}
+
+int64_t srx_selective_scan_workspace(srx_handle_t h, const srx_scan_t* s, int64_t n_utts, int64_t n_frames) {
+    return workspace_bytes_for(h, s, n_utts, n_frames, false, "srx_selective_scan_workspace");
+}
+
+int64_t srx_selective_scan_backward_workspace(srx_handle_t h, const srx_scan_t* s, int64_t n_utts,
+                                              int64_t n_frames) {
+    return workspace_bytes_for(h, s, n_utts, n_frames, true, "srx_selective_scan_backward_workspace");
+}
+
+int srx_selective_scan(srx_handle_t h, const srx_scan_t* s, const srx_scan_inputs_t* in, int dtype,
+                       const int64_t* utt_offsets, int64_t n_utts, int64_t n_frames, const float* state_in,
+                       float* state_out, void* y, int64_t ld_y, float* saved, void* workspace,
+                       int64_t workspace_bytes, void* stream) {
+    const char* who = "srx_selective_scan";
+    int rc = check_scan(h, s, n_utts, n_frames, who);
+    if (rc) return rc;
+    if ((rc = check_inputs(s, in, dtype, n_frames, who))) return rc;
+    if (n_utts == 0) return SRX_OK;
+    SRX_REQUIRE(utt_offsets != nullptr, "%s: NULL utterance offsets", who);
+    SRX_REQUIRE(n_frames == 0 || y != nullptr, "%s: NULL y", who);
+    SRX_REQUIRE(n_frames == 0 || ld_y >= s->n_channels, "%s: a row pitch is smaller than its row", who);
+    ScanParams p = params_for(h, s, n_utts, n_frames);
+    const int64_t need = carve(p, false, workspace);
+    SRX_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need),
+                "%s: workspace of %lld bytes, %lld are needed", who, (long long)workspace_bytes, (long long)need);
+    take_inputs(p, in);
+    p.off = utt_offsets;
+    p.state_in = state_in;
+    p.state_out = state_out;
+    p.y = y;
+    p.ld_y = ld_y;
+    p.saved = saved;
+    DeviceGuard guard(h->device);
+    if (guard.rc) return guard.rc;
+    return run(p, dtype, false, (hipStream_t)stream);
+}
+
+int srx_selective_scan_step(srx_handle_t h, const srx_scan_t* s, const srx_scan_inputs_t* in, int dtype,
+                            int64_t n_rows, float* state, void* y, int64_t ld_y, void* stream) {
+    const char* who = "srx_selective_scan_step";
+    int rc = check_scan(h, s, n_rows, n_rows, who);
+    if (rc) return rc;
+    if ((rc = check_inputs(s, in, dtype, n_rows, who))) return rc;
+    if (n_rows == 0) return SRX_OK;
+    SRX_REQUIRE(state != nullptr && y != nullptr, "%s: NULL state or y", who);
+    SRX_REQUIRE(ld_y >= s->n_channels, "%s: a row pitch is smaller than its row", who);
+    ScanParams p = params_for(h, s, n_rows, n_rows);
+    take_inputs(p, in);
+    p.y = y;
+    p.ld_y = ld_y;
+    DeviceGuard guard(h->device);
+    if (guard.rc) return guard.rc;
+    switch (dtype) {
+        case SRX_F32: return scan_step_run<float>(p, state, n_rows, (hipStream_t)stream);
+        case SRX_BF16: return scan_step_run<__bf16>(p, state, n_rows, (hipStream_t)stream);
+        default: return scan_step_run<_Float16>(p, state, n_rows, (hipStream_t)stream);
+    }
+}
+
+int srx_selective_scan_backward(srx_handle_t h, const srx_scan_t* s, const srx_scan_inputs_t* in, int dtype,
+                                const int64_t* utt_offsets, int64_t n_utts, int64_t n_frames,
+                                const float* saved, const void* dy, int64_t ld_dy, const float* dstate_out,
+                                const srx_scan_gradients_t* grads, float* dA, float* dskip, float* ddt_bias,
+                                float* dstate_in, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* who = "srx_selective_scan_backward";
+    int rc = check_scan(h, s, n_utts, n_frames, who);
+    if (rc) return rc;
+    if ((rc = check_inputs(s, in, dtype, n_frames, who))) return rc;
+    const int64_t c = s->n_channels, bc = (int64_t)s->n_groups * s->n_states;
+    SRX_REQUIRE(grads != nullptr && dA != nullptr, "%s: NULL gradients", who);
+    SRX_REQUIRE((dskip != nullptr) == (s->skip != nullptr) && (ddt_bias != nullptr) == (s->dt_bias != nullptr),
+                "%s: dskip / ddt_bias must be given exactly where skip / dt_bias are", who);
+    SRX_REQUIRE(n_utts == 0 || utt_offsets != nullptr, "%s: NULL utterance offsets", who);
+    if (n_frames > 0) {
+        SRX_REQUIRE(saved != nullptr && dy != nullptr, "%s: NULL saved or dy", who);
+        SRX_REQUIRE(grads->dx && grads->ddt && grads->dB && grads->dC &&
+                        (in->gate == nullptr) == (grads->dgate == nullptr),
+                    "%s: NULL gradient of an input (dgate must be given exactly where gate is)", who);
+        SRX_REQUIRE(ld_dy >= c && grads->ld_dx >= c && grads->ld_ddt >= c && grads->ld_dB >= bc &&
+                        grads->ld_dC >= bc && (in->gate == nullptr || grads->ld_dgate >= c),
+                    "%s: a row pitch is smaller than its row", who);
+    }
+    ScanParams p = params_for(h, s, n_utts, n_frames);
+    const int64_t need = carve(p, true, workspace);
+    SRX_REQUIRE(workspace != nullptr && workspace_bytes >= need,
+                "%s: workspace of %lld bytes, %lld are needed", who, (long long)workspace_bytes, (long long)need);
+    take_inputs(p, in);
+    p.off = utt_offsets;
+    p.saved = const_cast<float*>(saved);     // (the backward kernels only read it)
+    p.dy = dy;
+    p.ld_dy = ld_dy;
+    p.dx = grads->dx;
+    p.ddt = grads->ddt;
+    p.dB = grads->dB;
+    p.dC = grads->dC;
+    p.dgate = grads->dgate;
+    p.ld_dx = grads->ld_dx;
+    p.ld_ddt = grads->ld_ddt;
+    p.ld_dB = grads->ld_dB;
+    p.ld_dC = grads->ld_dC;
+    p.ld_dgate = grads->ld_dgate;
+    p.dA = dA;
+    p.dskip = dskip;
+    p.dbias = ddt_bias;
+    p.dstate_in = dstate_in;
+    p.dstate_out = dstate_out;
+    DeviceGuard guard(h->device);
+    if (guard.rc) return guard.rc;
+    return run(p, dtype, true, (hipStream_t)stream);
+}
+
+}  // extern "C"
