@@ -11,7 +11,8 @@ namespace srx_frames {
 
 template <typename T, int V>
 struct Pack {
-    T v[V];
+    typedef T Vec __attribute__((ext_vector_type(V)));
+    Vec v;
 };
 
 // V neighbouring elements as one memory instruction: gfx950 takes global accesses at any
@@ -19,12 +20,12 @@ struct Pack {
 template <int V, typename T>
 __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
     Pack<T, V> r;
-    __builtin_memcpy(&r, (const void*)p, sizeof(r));
+    __builtin_memcpy(&r.v, (const void*)p, V * sizeof(T));
     return r;
 }
 template <int V, typename T>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
-    __builtin_memcpy((void*)p, &v, sizeof(v));
+    __builtin_memcpy((void*)p, &v.v, V * sizeof(T));
 }
 // The first `n` (<= V) of V neighbouring elements, zeros behind them.
 template <int V, typename T>
@@ -96,8 +97,13 @@ __device__ __forceinline__ float rows_sum(float a, float b) {
 }
 template <int CTRL>
 __device__ __forceinline__ float dpp_mov(float v) {
-    const int i = __float_as_int(v);
-    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// Sum over four neighbouring lanes, in all of them.
+__device__ __forceinline__ float quad_sum(float v) {
+    v += dpp_mov<0xB1>(v);      // quad_perm [1,0,3,2]
+    v += dpp_mov<0x4E>(v);      // quad_perm [2,3,0,1]
+    return v;
 }
 // Sum over the 16 lanes of a row, in all of them.
 __device__ __forceinline__ float row16_sum(float v) {

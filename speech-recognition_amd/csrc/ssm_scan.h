@@ -35,6 +35,7 @@ struct ScanParams {
     int per_group;           // channels of a group
     int group_blocks;        // channel blocks (of 16 R) of a group
     int blocks;              // of all groups
+    int wide;                // R: channels of a lane
     // frames
     const int64_t* off;
     int64_t utts, frames;
@@ -100,27 +101,64 @@ __device__ __forceinline__ bool scan_unit(const ScanParams& p, int64_t unit, Sca
     return true;
 }
 
-// Channels of a wave's block, and where they are.
-template <int R, int S>
+// Channels of a wave's block, and where they are.  QUADS false: the four rows of 16 lanes hold the four groups of
+// states, lane 16 row + col; true: four neighbouring lanes do, lane 4 col + row.
+template <int R, int S, bool QUADS>
 struct ScanLane {
     static constexpr int kChannels = 16 * R, kStates = 4 * S;
     int lane, row, col;
     int group, channel, left;    // first channel of this lane, how many of its R exist
+    int end;                     // the group's last channel
     int state;                   // first state of this lane
+    bool full;                   // the block has all its channels (the same for the whole wave)
     __device__ __forceinline__ ScanLane(const ScanParams& p, int block) {
         lane = threadIdx.x & 63;
-        row = lane >> 4;
-        col = lane & 15;
+        row = QUADS ? lane & 3 : lane >> 4;
+        col = QUADS ? lane >> 2 : lane & 15;
         group = block / p.group_blocks;
-        const int base = (block - group * p.group_blocks) * kChannels + col * R;
+        const int first = (block - group * p.group_blocks) * kChannels, base = first + col * R;
         channel = group * p.per_group + base;
         left = min(max(p.per_group - base, 0), R);
+        end = (group + 1) * p.per_group - 1;
         state = row * S;
+        full = first + kChannels <= p.per_group;
+    }
+    // R neighbouring values of a frame's row, `at` the address of this lane's first.  Without them all the last one
+    // stands in for those that do not exist: no branch, nothing behind the row is touched.
+    template <typename T>
+    __device__ __forceinline__ Pack<T, R> load(const T* at, bool fast) const {
+        if (fast) return load_pack<R>(at);
+        Pack<T, R> v;
+#pragma unroll
+        for (int r = 0; r < R; ++r) v.v[r] = at[min(channel + r, end) - channel];
+        return v;
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(T* at, const Pack<T, R>& v) const {
+        if (full) {
+            store_pack(at, v);
+            return;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r < left) at[r] = v.v[r];
     }
 };
+// S states of a frame's B or C from state s0 on, zeros for those that do not exist.
+template <int S, typename T>
+__device__ __forceinline__ Pack<T, S> scan_load_bc(const T* at, int s0, int states, bool fast) {
+    if (fast) return load_pack<S>(at);
+    Pack<T, S> v;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const T x = at[min(s0 + s, states - 1) - s0];
+        v.v[s] = s0 + s < states ? x : (T)0.0f;
+    }
+    return v;
+}
 
-template <int R, int S>
-__device__ __forceinline__ void scan_load_states(const float* from, const ScanParams& p, const ScanLane<R, S>& w,
+template <int R, int S, bool Q>
+__device__ __forceinline__ void scan_load_states(const float* from, const ScanParams& p, const ScanLane<R, S, Q>& w,
                                                  int64_t utt, float (&h)[R][S]) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -129,8 +167,8 @@ __device__ __forceinline__ void scan_load_states(const float* from, const ScanPa
             h[r][s] = from != nullptr && r < w.left && w.state + s < p.states
                           ? from[(utt * p.channels + w.channel + r) * p.states + w.state + s] : 0.0f;
 }
-template <int R, int S>
-__device__ __forceinline__ void scan_store_states(float* to, const ScanParams& p, const ScanLane<R, S>& w,
+template <int R, int S, bool Q>
+__device__ __forceinline__ void scan_store_states(float* to, const ScanParams& p, const ScanLane<R, S, Q>& w,
                                                   int64_t utt, const float (&h)[R][S]) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -139,10 +177,11 @@ __device__ __forceinline__ void scan_store_states(float* to, const ScanParams& p
             if (r < w.left && w.state + s < p.states)
                 to[(utt * p.channels + w.channel + r) * p.states + w.state + s] = h[r][s];
 }
-// The same in the lanes' own order (whole lines per instruction, padded channels and states included).
-template <int R, int S>
-__device__ __forceinline__ void scan_load_lanes(const float* from, int64_t at, int lane, float (&h)[R][S]) {
-    const float* base = from + (at * (R * S / 4) * 64 + lane) * 4;
+// The same in an order of their own, in which an instruction of the wave covers whole lines: for every four
+// values of a lane, lane 16 row + col (padded channels and states included).
+template <int R, int S, bool Q>
+__device__ __forceinline__ void scan_load_lanes(const float* from, int64_t at, const ScanLane<R, S, Q>& w, float (&h)[R][S]) {
+    const float* base = from + (at * (R * S / 4) * 64 + w.row * 16 + w.col) * 4;
 #pragma unroll
     for (int q = 0; q < R * S / 4; ++q) {
         const Pack<float, 4> v = load_pack<4>(base + q * 256);
@@ -150,9 +189,9 @@ __device__ __forceinline__ void scan_load_lanes(const float* from, int64_t at, i
         for (int k = 0; k < 4; ++k) h[(q * 4 + k) / S][(q * 4 + k) % S] = v.v[k];
     }
 }
-template <int R, int S>
-__device__ __forceinline__ void scan_store_lanes(float* to, int64_t at, int lane, const float (&h)[R][S]) {
-    float* base = to + (at * (R * S / 4) * 64 + lane) * 4;
+template <int R, int S, bool Q>
+__device__ __forceinline__ void scan_store_lanes(float* to, int64_t at, const ScanLane<R, S, Q>& w, const float (&h)[R][S]) {
+    float* base = to + (at * (R * S / 4) * 64 + w.row * 16 + w.col) * 4;
 #pragma unroll
     for (int q = 0; q < R * S / 4; ++q) {
         Pack<float, 4> v;
@@ -166,8 +205,8 @@ __device__ __forceinline__ int64_t scan_slot(const ScanUnit& u, int64_t t) {
 }
 
 // A log2(e), so that the decay is one product and the hardware's 2^x.
-template <int R, int S>
-__device__ __forceinline__ void scan_load_A(const ScanParams& p, const ScanLane<R, S>& w, float (&A2)[R][S]) {
+template <int R, int S, bool Q>
+__device__ __forceinline__ void scan_load_A(const ScanParams& p, const ScanLane<R, S, Q>& w, float (&A2)[R][S]) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -178,23 +217,80 @@ __device__ __forceinline__ void scan_load_A(const ScanParams& p, const ScanLane<
 
 // ---- forward ------------------------------------------------------------------------------
 
-// A tile of frames on its way from memory: row g of the wave has frames 4 i + g.
+// A tile of frames on its way from memory: row g of the wave has frames 4 i + g.  Addresses advance with the tiles.
 template <typename T, int R, int S, bool GATE, bool WITH_Y>
 struct ScanTileRaw {
     Pack<T, R> x[4], dt[4], z[4];
     Pack<T, S> b, c;
-    __device__ __forceinline__ void load(const ScanParams& p, const ScanLane<R, S>& w, int64_t t0, int64_t last) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t t = min(t0 + 4 * i + w.row, last - 1);      // behind the last frame: it again, unused
-            x[i] = load_some<R>((const T*)p.x + t * p.ld_x + w.channel, w.left);
-            dt[i] = load_some<R>((const T*)p.dt + t * p.ld_dt + w.channel, w.left);
-            if (GATE && WITH_Y) z[i] = load_some<R>((const T*)p.gate + t * p.ld_gate + w.channel, w.left);
-        }
-        const int64_t t = min(t0 + (w.lane >> 2), last - 1);
+};
+template <typename T, int R, int S, bool GATE, bool WITH_Y>
+struct ScanTileReader {
+    const T *x, *dt, *z, *b, *c;
+    int64_t ld_x, ld_dt, ld_z, ld_b, ld_c;
+    bool all_states;
+    __device__ __forceinline__ ScanTileReader(const ScanParams& p, const ScanLane<R, S, false>& w, int64_t first) {
+        ld_x = p.ld_x;
+        ld_dt = p.ld_dt;
+        ld_z = p.ld_gate;
+        ld_b = p.ld_B;
+        ld_c = p.ld_C;
+        const int64_t t = first + w.row, tb = first + (w.lane >> 2);
+        const int64_t s0 = (int64_t)w.group * p.states + (w.lane & 3) * S;
+        x = (const T*)p.x + t * ld_x + w.channel;
+        dt = (const T*)p.dt + t * ld_dt + w.channel;
+        z = GATE && WITH_Y ? (const T*)p.gate + t * ld_z + w.channel : nullptr;
+        b = (const T*)p.B + tb * ld_b + s0;
+        c = WITH_Y ? (const T*)p.C + tb * ld_c + s0 : nullptr;
+        all_states = p.states == 4 * S;
+    }
+    // The next `frames` frames (at least one): a whole tile without a branch, a shorter one with its last frame in
+    // place of those behind it, which are not used.
+    __device__ __forceinline__ void next(const ScanParams& p, const ScanLane<R, S, false>& w, int64_t frames,
+                                         ScanTileRaw<T, R, S, GATE, WITH_Y>& to) {
         const int s0 = (w.lane & 3) * S;
-        b = load_some<S>((const T*)p.B + t * p.ld_B + (int64_t)w.group * p.states + s0, p.states - s0);
-        if (WITH_Y) c = load_some<S>((const T*)p.C + t * p.ld_C + (int64_t)w.group * p.states + s0, p.states - s0);
+        if (frames >= kScanTile && w.full) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                to.x[i] = load_pack<R>(x + 4 * i * ld_x);
+                to.dt[i] = load_pack<R>(dt + 4 * i * ld_dt);
+                if (GATE && WITH_Y) to.z[i] = load_pack<R>(z + 4 * i * ld_z);
+            }
+            to.b = scan_load_bc<S>(b, s0, p.states, all_states);
+            if (WITH_Y) to.c = scan_load_bc<S>(c, s0, p.states, all_states);
+        } else {
+            const int last = (int)min(frames, (int64_t)kScanTile) - 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t t = min(4 * i + w.row, last) - w.row;
+                to.x[i] = w.load(x + t * ld_x, w.full);
+                to.dt[i] = w.load(dt + t * ld_dt, w.full);
+                if (GATE && WITH_Y) to.z[i] = w.load(z + t * ld_z, w.full);
+            }
+            const int64_t t = min(w.lane >> 2, last) - (w.lane >> 2);
+            to.b = scan_load_bc<S>(b + t * ld_b, s0, p.states, all_states);
+            if (WITH_Y) to.c = scan_load_bc<S>(c + t * ld_c, s0, p.states, all_states);
+        }
+        x += kScanTile * ld_x;
+        dt += kScanTile * ld_dt;
+        if (GATE && WITH_Y) z += kScanTile * ld_z;
+        b += kScanTile * ld_b;
+        if (WITH_Y) c += kScanTile * ld_c;
+    }
+};
+
+// A frame's values for one lane, from the wave's LDS.
+template <int R, int S>
+struct ScanFrame {
+    Pack<float, R> d, du, q;
+    Pack<float, S> b, c;
+    template <bool WITH_B, bool WITH_C, bool QUADS>
+    __device__ __forceinline__ void load(const ScanLane<R, S, QUADS>& w, int j, const float* sD, const float* sU,
+                                         const float* sP, const float* sB, const float* sC) {
+        d = load_pack<R>(sD + j * (16 * R) + w.col * R);
+        if (sU != nullptr) du = load_pack<R>(sU + j * (16 * R) + w.col * R);
+        if (sP != nullptr) q = load_pack<R>(sP + j * (16 * R) + w.col * R);
+        if (WITH_B) b = load_pack<S>(sB + j * (4 * S) + w.state);
+        if (WITH_C) c = load_pack<S>(sC + j * (4 * S) + w.state);
     }
 };
 
@@ -202,7 +298,7 @@ struct ScanTileRaw {
 template <typename T, int R, int S, bool GATE, int MODE>
 __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParams p) {
     constexpr int CH = 16 * R, NS = 4 * S, TILE = kScanTile;
-    __shared__ float lds[kScanWaves][2 * TILE * (CH + NS)];
+    __shared__ __align__(16) float lds[kScanWaves][2 * TILE * (CH + NS)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* sD = lds[wave];
     float* sU = sD + TILE * CH;
@@ -214,7 +310,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
         const int block = (int)(task - unit * across) * kScanWaves + wave;
         ScanUnit u;
         if (block >= p.blocks || !scan_unit(p, unit, u)) continue;
-        const ScanLane<R, S> w(p, block);
+        const ScanLane<R, S, false> w(p, block);
         float A2[R][S], h[R][S], bias[R], skip[R], total[R];
         scan_load_A(p, w, A2);
 #pragma unroll
@@ -225,7 +321,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
         }
         const int64_t place = unit * p.blocks + block;
         if (MODE == 0) {
-            if (p.segment != 0) scan_load_lanes(p.seg_state, place, w.lane, h);
+            if (p.segment != 0) scan_load_lanes(p.seg_state, place, w, h);
             else scan_load_states(p.state_in, p, w, u.utt, h);
         } else {
 #pragma unroll
@@ -233,14 +329,21 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
 #pragma unroll
                 for (int s = 0; s < S; ++s) h[r][s] = 0.0f;
         }
+        const int64_t frames = u.last - u.first;
+        ScanTileReader<T, R, S, GATE, MODE == 0> reader(p, w, u.first);
         ScanTileRaw<T, R, S, GATE, MODE == 0> now, next;
-        if (u.first < u.last) now.load(p, w, u.first, u.last);
-        for (int64_t t0 = u.first; t0 < u.last; t0 += TILE) {
-            if (t0 + TILE < u.last) next.load(p, w, t0 + TILE, u.last);
+        T* y = (T*)p.y + (u.first + w.row) * p.ld_y + w.channel;
+        float* saved = nullptr;
+        if (MODE == 0 && p.saved != nullptr)
+            saved = p.saved + (scan_slot(u, u.first) * p.blocks + block) * (R * S * 64);
+        if (frames > 0) reader.next(p, w, frames, now);
+        for (int64_t done = 0; done < frames; done += TILE) {
+            const int here = (int)min(frames - done, (int64_t)TILE);       // frames of this tile
+            if (done + TILE < frames) reader.next(p, w, frames - done - TILE, next);
             wave_lds_fence();                            // the last tile has been read
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool live = t0 + 4 * i + w.row < u.last;
+                const bool live = 4 * i + w.row < here;
                 Pack<float, R> d, du;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
@@ -264,35 +367,38 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
                 if (MODE == 0) store_pack(sC + w.lane * S, c);
             }
             wave_lds_fence();
+            ScanFrame<R, S> f;
+            f.template load<true, MODE == 0>(w, 0, sD, sU, nullptr, sB, sC);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (MODE == 0 && i % 2 == 0 && p.saved != nullptr && t0 + 4 * i < u.last)
-                    scan_store_lanes(p.saved, scan_slot(u, t0 + 4 * i) * p.blocks + block, w.lane, h);
-                float y[4][R];
+                if (MODE == 0 && i % 2 == 0 && saved != nullptr && 4 * i < here) {
+                    scan_store_lanes(saved, 0, w, h);
+                    saved += (int64_t)p.blocks * (R * S * 64);
+                }
+                float part[4][R];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const Pack<float, R> d = load_pack<R>(sD + (4 * i + j) * CH + w.col * R);
-                    const Pack<float, R> du = load_pack<R>(sU + (4 * i + j) * CH + w.col * R);
-                    const Pack<float, S> b = load_pack<S>(sB + (4 * i + j) * NS + w.state);
-                    Pack<float, S> c;
-                    if (MODE == 0) c = load_pack<S>(sC + (4 * i + j) * NS + w.state);
+                    ScanFrame<R, S> ahead;               // the next frame's values are read while this one's are used
+                    if (4 * i + j + 1 < TILE) ahead.template load<true, MODE == 0>(w, 4 * i + j + 1, sD, sU, nullptr, sB, sC);
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        y[j][r] = 0.0f;
+                        part[j][r] = 0.0f;
 #pragma unroll
                         for (int s = 0; s < S; ++s) {
-                            const float a = __builtin_amdgcn_exp2f(d.v[r] * A2[r][s]);
-                            h[r][s] = fmaf(a, h[r][s], du.v[r] * b.v[s]);
-                            if (MODE == 0) y[j][r] = fmaf(c.v[s], h[r][s], y[j][r]);
+                            const float a = __builtin_amdgcn_exp2f(f.d.v[r] * A2[r][s]);
+                            h[r][s] = fmaf(a, h[r][s], f.du.v[r] * f.b.v[s]);
+                            if (MODE == 0) part[j][r] = fmaf(f.c.v[s], h[r][s], part[j][r]);
                         }
                     }
+                    f = ahead;
+                    __builtin_amdgcn_sched_barrier(0);   // (no more than that: registers)
                 }
                 if (MODE == 0) {
                     // the four rows' shares added up; row g is left with frame 4 i + g
                     Pack<T, R> out;
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        float v = rows_sum(halves_sum(y[0][r], y[2][r]), halves_sum(y[1][r], y[3][r]));
+                        float v = rows_sum(halves_sum(part[0][r], part[2][r]), halves_sum(part[1][r], part[3][r]));
                         v = fmaf(skip[r], (float)now.x[i].v[r], v);
                         if (GATE) {
                             const float z = (float)now.z[i].v[r];
@@ -300,8 +406,8 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
                         }
                         out.v[r] = (T)v;                 // the one rounding to the output's type
                     }
-                    const int64_t t = t0 + 4 * i + w.row;
-                    if (t < u.last) store_some((T*)p.y + t * p.ld_y + w.channel, out, w.left);
+                    if (4 * i + w.row < here) w.store(y, out);
+                    y += 4 * p.ld_y;
                 }
             }
             now = next;
@@ -309,7 +415,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
         if (MODE == 0) {
             if (p.state_out != nullptr && u.tail) scan_store_states(p.state_out, p, w, u.utt, h);
         } else {
-            scan_store_lanes(p.seg_state, place, w.lane, h);
+            scan_store_lanes(p.seg_state, place, w, h);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const float v = rows_sum(total[r], total[r]);
@@ -327,34 +433,80 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
 
 // The pieces of an utterance joined: seg_state holds what each piece's frames add to the state
 // (REVERSE: to the gradient of the state before it), and is replaced by the state that enters the piece
-// (the gradient that enters it from behind).  One wave per utterance and channel block walks over the
-// pieces; its loads do not depend on one another.
+// (the gradient that enters it from behind).  A workgroup has four values of each lane of one channel block;
+// its waves take a run of pieces each, add them up from zero, hand the result to the waves behind them through LDS, and
+// walk over their run again with the state that enters it.
+constexpr int kJoinWaves = 16;
 template <int R, int S, bool REVERSE>
-__global__ __launch_bounds__(64) void scan_join_kernel(ScanParams p) {
-    constexpr int CH = 16 * R;
-    for (int64_t task = blockIdx.x; task < p.utts * p.blocks; task += gridDim.x) {
-        const int64_t utt = task / p.blocks;
-        const int block = (int)(task - utt * p.blocks);
-        const ScanLane<R, S> w(p, block);
-        float A2[R][S], h[R][S];
-        scan_load_A(p, w, A2);
-        scan_load_states(REVERSE ? p.dstate_out : p.state_in, p, w, utt, h);
+__global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanParams p) {
+    constexpr int CH = 16 * R, QUADS = R * S / 4, AHEAD = 4;
+    __shared__ float lds[kJoinWaves][2][64][4];
+    const int wave = threadIdx.x >> 6;
+    for (int64_t task = blockIdx.x; task < p.utts * p.blocks * QUADS; task += gridDim.x) {
+        const int q = (int)(task % QUADS);
+        const int64_t rest = task / QUADS, utt = rest / p.blocks;
+        const int block = (int)(rest - utt * p.blocks);
+        const ScanLane<R, S, false> w(p, block);
+        float A2[4], h[4], decay[4];
+        const float* enter = REVERSE ? p.dstate_out : p.state_in;
+        float from[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = (q * 4 + k) / S, s = w.state + (q * 4 + k) % S;
+            const bool in = r < w.left && s < p.states;
+            A2[k] = in ? p.A[(int64_t)(w.channel + r) * p.states + s] * 1.44269504088896341f : 0.0f;
+            from[k] = in && enter != nullptr ? enter[(utt * p.channels + w.channel + r) * p.states + s] : 0.0f;
+            h[k] = decay[k] = 0.0f;
+        }
         int64_t begin, end;
         scan_bounds(p, utt, begin, end);
         const int64_t base = begin / p.segment + utt;
         const int64_t pieces = max((end - begin + p.segment - 1) / p.segment, (int64_t)1);
-        for (int64_t k = 0; k < pieces; ++k) {
-            const int64_t place = (base + (REVERSE ? pieces - 1 - k : k)) * p.blocks + block;
-            float own[R][S];
-            scan_load_lanes(p.seg_state, place, w.lane, own);
-            const Pack<float, R> sum = load_pack<R>(p.seg_sum + place * CH + w.col * R);
-            scan_store_lanes(p.seg_state, place, w.lane, h);
+        const int64_t run = (pieces + kJoinWaves - 1) / kJoinWaves;
+        const int64_t k0 = min(wave * run, pieces), k1 = min(k0 + run, pieces);
+        auto place = [&](int64_t k) { return (base + (REVERSE ? pieces - 1 - k : k)) * p.blocks + block; };
+        auto walk = [&](bool write) {
+            for (int64_t k = k0; k < k1; k += AHEAD) {
+                Pack<float, 4> own[AHEAD];
+                float sum[AHEAD][4];
 #pragma unroll
-            for (int r = 0; r < R; ++r)
+                for (int a = 0; a < AHEAD; ++a) {
+                    const int64_t at = place(min(k + a, k1 - 1));
+                    own[a] = load_pack<4>(p.seg_state + ((at * QUADS + q) * 64 + w.lane) * 4);
 #pragma unroll
-                for (int s = 0; s < S; ++s)
-                    h[r][s] = fmaf(__builtin_amdgcn_exp2f(sum.v[r] * A2[r][s]), h[r][s], own[r][s]);
+                    for (int e = 0; e < 4; ++e) sum[a][e] = p.seg_sum[at * CH + w.col * R + (q * 4 + e) / S];
+                }
+#pragma unroll
+                for (int a = 0; a < AHEAD; ++a) {
+                    if (k + a >= k1) break;
+                    if (write) {
+                        Pack<float, 4> v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v.v[e] = h[e];
+                        store_pack(p.seg_state + ((place(k + a) * QUADS + q) * 64 + w.lane) * 4, v);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        h[e] = fmaf(__builtin_amdgcn_exp2f(sum[a][e] * A2[e]), h[e], own[a].v[e]);
+                        decay[e] += sum[a][e];
+                    }
+                }
+            }
+        };
+        walk(false);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            lds[wave][0][w.lane][e] = h[e];
+            lds[wave][1][w.lane][e] = decay[e];
+            h[e] = from[e];
         }
+        __syncthreads();
+        for (int before = 0; before < wave; ++before)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                h[e] = fmaf(__builtin_amdgcn_exp2f(lds[before][1][w.lane][e] * A2[e]), h[e], lds[before][0][w.lane][e]);
+        walk(true);
+        __syncthreads();                                 // (the next task's results go to the same place)
     }
 }
 
@@ -362,51 +514,94 @@ __global__ __launch_bounds__(64) void scan_join_kernel(ScanParams p) {
 //
 // Backwards in time, g_{t-1} = exp(d_t A) (dp_t C_t + g_t) is what the loss owes to the state before
 // frame t.  The states themselves are saved by the forward pass before every eighth frame and computed
-// again from there, in registers, four frames at a time: the first four frames' states of an
-// octet are run through once to reach the second four.  Sums over the states (dd, dx, the gated sum)
-// cross the rows of a wave, sums over the channels (dB, dC) its columns.
+// again from there, in registers.  Sums over the states (dd, dx, the gated sum) cross the four lanes that share
+// channels, here neighbours (two quad permutations per sum); sums over the channels (dB, dC) cross the 16 lanes that
+// share states: the first two of their four steps exchange whole halves and rows between two
+// registers, so that each step halves the number of registers too.
 
 template <typename T, int R, int S, bool GATE>
 struct ScanOctetRaw {
     Pack<T, R> x[2], dt[2], z[2], dy[2];
     Pack<T, S> bc;               // lanes 0 .. 31: B, lanes 32 .. 63: C
-    __device__ __forceinline__ void load(const ScanParams& p, const ScanLane<R, S>& w, int64_t t0, int64_t last) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t t = min(t0 + 4 * i + w.row, last - 1);
-            x[i] = load_some<R>((const T*)p.x + t * p.ld_x + w.channel, w.left);
-            dt[i] = load_some<R>((const T*)p.dt + t * p.ld_dt + w.channel, w.left);
-            if (GATE) z[i] = load_some<R>((const T*)p.gate + t * p.ld_gate + w.channel, w.left);
-            dy[i] = load_some<R>((const T*)p.dy + t * p.ld_dy + w.channel, w.left);
-        }
-        const int64_t t = min(t0 + ((w.lane & 31) >> 2), last - 1);
+};
+template <typename T, int R, int S, bool GATE>
+struct ScanOctetReader {
+    const T *x, *dt, *z, *dy, *bc;
+    int64_t ld_x, ld_dt, ld_z, ld_dy, ld_bc;
+    bool all_states;
+    // `first`: the first frame of the octet that is read first; later ones lie before it
+    __device__ __forceinline__ ScanOctetReader(const ScanParams& p, const ScanLane<R, S, true>& w, int64_t first) {
+        ld_x = p.ld_x;
+        ld_dt = p.ld_dt;
+        ld_z = p.ld_gate;
+        ld_dy = p.ld_dy;
+        ld_bc = w.lane < 32 ? p.ld_B : p.ld_C;
+        const int64_t t = first + w.row;
+        x = (const T*)p.x + t * ld_x + w.channel;
+        dt = (const T*)p.dt + t * ld_dt + w.channel;
+        z = GATE ? (const T*)p.gate + t * ld_z + w.channel : nullptr;
+        dy = (const T*)p.dy + t * ld_dy + w.channel;
+        bc = (const T*)(w.lane < 32 ? p.B : p.C) + (first + ((w.lane & 31) >> 2)) * ld_bc + (int64_t)w.group * p.states +
+             (w.lane & 3) * S;
+        all_states = p.states == 4 * S;
+    }
+    __device__ __forceinline__ void next(const ScanParams& p, const ScanLane<R, S, true>& w, int frames,
+                                         ScanOctetRaw<T, R, S, GATE>& to) {
         const int s0 = (w.lane & 3) * S;
-        const T* from = w.lane < 32 ? (const T*)p.B + t * p.ld_B : (const T*)p.C + t * p.ld_C;
-        bc = load_some<S>(from + (int64_t)w.group * p.states + s0, p.states - s0);
+        if (frames >= kScanSaveEvery && w.full) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                to.x[i] = load_pack<R>(x + 4 * i * ld_x);
+                to.dt[i] = load_pack<R>(dt + 4 * i * ld_dt);
+                if (GATE) to.z[i] = load_pack<R>(z + 4 * i * ld_z);
+                to.dy[i] = load_pack<R>(dy + 4 * i * ld_dy);
+            }
+            to.bc = scan_load_bc<S>(bc, s0, p.states, all_states);
+        } else {
+            const int last = min(frames, kScanSaveEvery) - 1;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int64_t t = min(4 * i + w.row, last) - w.row;
+                to.x[i] = w.load(x + t * ld_x, w.full);
+                to.dt[i] = w.load(dt + t * ld_dt, w.full);
+                if (GATE) to.z[i] = w.load(z + t * ld_z, w.full);
+                to.dy[i] = w.load(dy + t * ld_dy, w.full);
+            }
+            const int at = (w.lane & 31) >> 2;
+            to.bc = scan_load_bc<S>(bc + (int64_t)(min(at, last) - at) * ld_bc, s0, p.states, all_states);
+        }
+        x -= kScanSaveEvery * ld_x;
+        dt -= kScanSaveEvery * ld_dt;
+        if (GATE) z -= kScanSaveEvery * ld_z;
+        dy -= kScanSaveEvery * ld_dy;
+        bc -= kScanSaveEvery * ld_bc;
     }
 };
 
-// The sum of v[r] over the four rows; row g gets that of r = g (R = 4), g / 2 (R = 2), 0 (R = 1).
-template <int R>
-__device__ __forceinline__ float scan_rows(const float (&v)[R]) {
-    if constexpr (R == 4) {
-        return rows_sum(halves_sum(v[0], v[2]), halves_sum(v[1], v[3]));
-    } else if constexpr (R == 2) {
-        const float a = halves_sum(v[0], v[1]);
-        return rows_sum(a, a);
-    } else {
-        const float a = halves_sum(v[0], v[0]);
-        return rows_sum(a, a);
+// Sums over the 16 lanes that share states: lane 4 col + row gets of (lanes 0 .. 31: b, lanes 32 .. 63: c) the values
+// odd S / 2 .. (odd rows of 16 lanes the second half of them; S = 1: all rows the one).
+template <int S>
+__device__ __forceinline__ void scan_sum_channels(const float (&b)[S], const float (&c)[S], float (&out)[S > 1 ? S / 2 : 1]) {
+    float half[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) half[s] = halves_sum(b[s], c[s]);
+#pragma unroll
+    for (int s = 0; s < (S > 1 ? S / 2 : 1); ++s) {
+        float v = rows_sum(half[s], half[S > 1 ? s + S / 2 : 0]);
+        v += dpp_mov<0x124>(v);     // row_ror:4
+        v += dpp_mov<0x128>(v);     // row_ror:8
+        out[s] = v;
     }
 }
 
 // MODE 0: the gradients.  MODE 1: only what a piece adds to the gradient of the state before it,
-// and the sum of its steps.
-template <typename T, int R, int S, bool GATE, int MODE>
+// and the sum of its steps.  SUB: frames whose states and decays are held at once, 8 or 4 (then the first four
+// frames are run through once to reach the second four).
+template <typename T, int R, int S, bool GATE, int MODE, int SUB>
 __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanParams p) {
     constexpr int CH = 16 * R, NS = 4 * S, TILE = kScanSaveEvery;
     constexpr float kLn2 = 0.693147180559945309f;
-    __shared__ float lds[kScanWaves][TILE * (6 * CH + 2 * NS) + 64 * (R * S + 2 * R)];
+    __shared__ __align__(16) float lds[kScanWaves][TILE * (6 * CH + 2 * NS) + (MODE == 0 ? 64 * (R * S + 2 * R) : 0)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* sD = lds[wave];               // steps
     float* sU = sD + TILE * CH;          // step times x
@@ -422,8 +617,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
         const int64_t part = task / across;
         const int block = (int)(task - part * across) * kScanWaves + wave;
         if (block >= p.blocks) continue;
-        const ScanLane<R, S> w(p, block);
-        const int owner = R == 4 ? w.row : R == 2 ? w.row >> 1 : 0;      // the channel whose sums this row gets
+        const ScanLane<R, S, true> w(p, block);
         float A2[R][S], bias[R], skip[R], dA[R][S], dskip[R], dbias[R], total[R];
         scan_load_A(p, w, A2);
 #pragma unroll
@@ -461,7 +655,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
             const int64_t place = unit * p.blocks + block;
             float g[R][S];
             if (MODE == 0) {
-                if (p.segment != 0) scan_load_lanes(p.seg_state, place, w.lane, g);
+                if (p.segment != 0) scan_load_lanes(p.seg_state, place, w, g);
                 else scan_load_states(p.dstate_out, p, w, u.utt, g);
             } else {
 #pragma unroll
@@ -472,30 +666,39 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                 }
             }
             const int64_t octets = (u.last - u.first + TILE - 1) / TILE;
+            const int64_t begin = u.first + (octets - 1) * TILE;           // of the last octet
+            ScanOctetReader<T, R, S, GATE> reader(p, w, begin);
+            ScanOctetRaw<T, R, S, GATE> now, next;
+            const float* saved = MODE == 0 ? p.saved + (scan_slot(u, begin) * p.blocks + block) * (R * S * 64) : nullptr;
+            float h0[R][S];
+            int frames = (int)(u.last - begin);
+            if (octets > 0) {
+                reader.next(p, w, frames, now);
+                if (MODE == 0) scan_load_lanes(saved, 0, w, h0);
+            }
+#pragma unroll 1
             for (int64_t o = octets - 1; o >= 0; --o) {
                 const int64_t t0 = u.first + o * TILE;
-                ScanOctetRaw<T, R, S, GATE> now;
-                now.load(p, w, t0, u.last);
-                float h0[R][S];
-                if (MODE == 0) scan_load_lanes(p.saved, scan_slot(u, t0) * p.blocks + block, w.lane, h0);
+                if (o > 0) reader.next(p, w, TILE, next);
                 wave_lds_fence();
                 float step[2][R], dp[2][R];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const bool live = t0 + 4 * i + w.row < u.last;
+                    const bool live = 4 * i + w.row < frames;
                     Pack<float, R> d, du, q;
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
+                        const bool in = live && r < w.left;      // (what does not exist adds nothing to dB and dC)
                         const float raw = (float)now.dt[i].v[r] + bias[r];
                         const float v = p.softplus ? softplus_f32(raw) : raw;
-                        d.v[r] = live ? v : 0.0f;
-                        du.v[r] = live ? v * (float)now.x[i].v[r] : 0.0f;
+                        d.v[r] = in ? v : 0.0f;
+                        du.v[r] = in ? v * (float)now.x[i].v[r] : 0.0f;
                         float dv = (float)now.dy[i].v[r];
                         if (GATE) {
                             const float z = (float)now.z[i].v[r];
                             dv *= z * sigmoid_f32(z);
                         }
-                        q.v[r] = live ? dv : 0.0f;
+                        q.v[r] = in ? dv : 0.0f;
                         step[i][r] = d.v[r];
                         dp[i][r] = q.v[r];
                         if (MODE == 1) total[r] += d.v[r];
@@ -514,101 +717,116 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                 if (MODE == 1) {
 #pragma unroll
                     for (int j = TILE - 1; j >= 0; --j) {
-                        const Pack<float, R> d = load_pack<R>(sD + j * CH + w.col * R);
-                        const Pack<float, R> q = load_pack<R>(sP + j * CH + w.col * R);
-                        const Pack<float, S> c = load_pack<S>(sC + j * NS + w.state);
+                        ScanFrame<R, S> f;
+                        f.template load<false, true>(w, j, sD, nullptr, sP, sB, sC);
 #pragma unroll
                         for (int r = 0; r < R; ++r)
 #pragma unroll
                             for (int s = 0; s < S; ++s)
-                                g[r][s] = fmaf(q.v[r], c.v[s], g[r][s]) * __builtin_amdgcn_exp2f(d.v[r] * A2[r][s]);
+                                g[r][s] = fmaf(f.q.v[r], f.c.v[s], g[r][s]) * __builtin_amdgcn_exp2f(f.d.v[r] * A2[r][s]);
                     }
+                    now = next;
+                    frames = TILE;
                     continue;
                 }
-                // states before the second four frames
                 float h4[R][S];
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int s = 0; s < S; ++s) h4[r][s] = h0[r][s];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const Pack<float, R> d = load_pack<R>(sD + j * CH + w.col * R);
-                    const Pack<float, R> du = load_pack<R>(sU + j * CH + w.col * R);
-                    const Pack<float, S> b = load_pack<S>(sB + j * NS + w.state);
+                if (SUB < TILE) {                                // states before the second four frames
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
-                        for (int s = 0; s < S; ++s)
-                            h4[r][s] = fmaf(__builtin_amdgcn_exp2f(d.v[r] * A2[r][s]), h4[r][s], du.v[r] * b.v[s]);
+                        for (int s = 0; s < S; ++s) h4[r][s] = h0[r][s];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        ScanFrame<R, S> f;
+                        f.template load<true, false>(w, j, sD, sU, nullptr, sB, sC);
+#pragma unroll
+                        for (int r = 0; r < R; ++r)
+#pragma unroll
+                            for (int s = 0; s < S; ++s)
+                                h4[r][s] = fmaf(__builtin_amdgcn_exp2f(f.d.v[r] * A2[r][s]), h4[r][s], f.du.v[r] * f.b.v[s]);
+                        if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
-#pragma unroll
-                for (int half = 1; half >= 0; --half) {
-                    float a[4][R][S], h[5][R][S];
+                float* to_bc = p.part_bc + ((int64_t)block * p.frames + t0) * 2 * NS + (w.lane >> 5) * NS + w.state +
+                               (S > 1 ? ((w.lane >> 4) & 1) * (S / 2) : 0);
+                const bool writes_bc = (w.lane & 12) == 0 && (S > 1 || (w.lane & 16) == 0);
+#pragma unroll 1
+                for (int half = TILE / SUB - 1; half >= 0; --half) {
+                    const int j0 = half * SUB;
+                    float a[SUB][R][S], h[SUB + 1][R][S];
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
-                        for (int s = 0; s < S; ++s) h[0][r][s] = half ? h4[r][s] : h0[r][s];
+                        for (int s = 0; s < S; ++s) h[0][r][s] = SUB < TILE && half ? h4[r][s] : h0[r][s];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int j = 4 * half + k;
-                        const Pack<float, R> d = load_pack<R>(sD + j * CH + w.col * R);
-                        const Pack<float, R> du = load_pack<R>(sU + j * CH + w.col * R);
-                        const Pack<float, S> b = load_pack<S>(sB + j * NS + w.state);
+                    for (int k = 0; k < SUB; ++k) {
+                        ScanFrame<R, S> f;
+                        f.template load<true, false>(w, j0 + k, sD, sU, nullptr, sB, sC);
 #pragma unroll
                         for (int r = 0; r < R; ++r)
 #pragma unroll
                             for (int s = 0; s < S; ++s) {
-                                a[k][r][s] = __builtin_amdgcn_exp2f(d.v[r] * A2[r][s]);
-                                h[k + 1][r][s] = fmaf(a[k][r][s], h[k][r][s], du.v[r] * b.v[s]);
+                                a[k][r][s] = __builtin_amdgcn_exp2f(f.d.v[r] * A2[r][s]);
+                                h[k + 1][r][s] = fmaf(a[k][r][s], h[k][r][s], f.du.v[r] * f.b.v[s]);
                             }
+                        if (k % 2 == 1) __builtin_amdgcn_sched_barrier(0);
                     }
+                    // the next octet's first states are on their way while this one's gradients are computed
+                    if (half == 0 && o > 0) {
+                        saved -= (int64_t)p.blocks * (R * S * 64);
+                        scan_load_lanes(saved, 0, w, h0);
+                    }
+                    ScanFrame<R, S> f;
+                    f.template load<true, true>(w, j0 + SUB - 1, sD, sU, sP, sB, sC);
 #pragma unroll
-                    for (int k = 3; k >= 0; --k) {
-                        const int j = 4 * half + k;
-                        const Pack<float, R> d = load_pack<R>(sD + j * CH + w.col * R);
-                        const Pack<float, R> du = load_pack<R>(sU + j * CH + w.col * R);
-                        const Pack<float, R> q = load_pack<R>(sP + j * CH + w.col * R);
-                        const Pack<float, S> b = load_pack<S>(sB + j * NS + w.state);
-                        const Pack<float, S> c = load_pack<S>(sC + j * NS + w.state);
-                        float su[R], sd[R], sy[R], db[S], dc[S];
+                    for (int k = SUB - 1; k >= 0; --k) {
+                        const int j = j0 + k;
+                        ScanFrame<R, S> ahead;
+                        if (k > 0) ahead.template load<true, true>(w, j - 1, sD, sU, sP, sB, sC);
+                        float db[S], dc[S];
+                        Pack<float, R> su, sd, sy;
 #pragma unroll
                         for (int s = 0; s < S; ++s) db[s] = dc[s] = 0.0f;
 #pragma unroll
                         for (int r = 0; r < R; ++r) {
-                            su[r] = sd[r] = sy[r] = 0.0f;
+                            float vu = 0.0f, vd = 0.0f, vy = 0.0f;
 #pragma unroll
                             for (int s = 0; s < S; ++s) {
-                                const float dh = fmaf(q.v[r], c.v[s], g[r][s]);
-                                dc[s] = fmaf(q.v[r], h[k + 1][r][s], dc[s]);
-                                if (GATE) sy[r] = fmaf(c.v[s], h[k + 1][r][s], sy[r]);
-                                db[s] = fmaf(dh, du.v[r], db[s]);
-                                su[r] = fmaf(dh, b.v[s], su[r]);
+                                const float dh = fmaf(f.q.v[r], f.c.v[s], g[r][s]);
+                                dc[s] = fmaf(f.q.v[r], h[k + 1][r][s], dc[s]);
+                                if (GATE) vy = fmaf(f.c.v[s], h[k + 1][r][s], vy);
+                                db[s] = fmaf(dh, f.du.v[r], db[s]);
+                                vu = fmaf(dh, f.b.v[s], vu);
                                 g[r][s] = dh * a[k][r][s];
                                 const float m = g[r][s] * h[k][r][s];
-                                sd[r] = fmaf(m, A2[r][s], sd[r]);
-                                dA[r][s] = fmaf(m, d.v[r], dA[r][s]);
+                                vd = fmaf(m, A2[r][s], vd);
+                                dA[r][s] = fmaf(m, f.d.v[r], dA[r][s]);
                             }
+                            su.v[r] = quad_sum(vu);
+                            sd.v[r] = quad_sum(vd);
+                            if (GATE) sy.v[r] = quad_sum(vy);
                         }
-                        const int at = j * CH + w.col * R + owner;
-                        oU[at] = scan_rows<R>(su);
-                        oD[at] = scan_rows<R>(sd);
-                        if (GATE) oY[at] = scan_rows<R>(sy);
-                        Pack<float, S> out;
+                        store_pack(oU + j * CH + w.col * R, su);        // (four lanes, the same values)
+                        store_pack(oD + j * CH + w.col * R, sd);
+                        if (GATE) store_pack(oY + j * CH + w.col * R, sy);
+                        constexpr int HALF = S > 1 ? S / 2 : 1;
+                        float sums[HALF];
+                        scan_sum_channels<S>(db, dc, sums);
+                        if (writes_bc && j < frames) {
+                            Pack<float, HALF> v;
 #pragma unroll
-                        for (int s = 0; s < S; ++s) {
-                            const float vb = row16_sum(db[s]), vc = row16_sum(dc[s]);
-                            out.v[s] = w.col == 0 ? vb : vc;
+                            for (int s = 0; s < HALF; ++s) v.v[s] = sums[s];
+                            store_pack(to_bc + j * 2 * NS, v);
                         }
-                        if (w.col < 2 && t0 + j < u.last)
-                            store_pack(p.part_bc + (((int64_t)block * p.frames + t0 + j) * 2 + w.col) * NS + w.state, out);
+                        f = ahead;
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
                 wave_lds_fence();
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int64_t t = t0 + 4 * i + w.row;
-                    const bool live = t < u.last;
+                    const bool live = 4 * i + w.row < frames;
                     const Pack<float, R> vu = load_pack<R>(oU + (4 * i + w.row) * CH + w.col * R);
                     const Pack<float, R> vd = load_pack<R>(oD + (4 * i + w.row) * CH + w.col * R);
                     Pack<float, R> vy;
@@ -632,29 +850,24 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                         }
                     }
                     if (live) {
-                        store_some((T*)p.dx + t * p.ld_dx + w.channel, dx, w.left);
-                        store_some((T*)p.ddt + t * p.ld_ddt + w.channel, ddt, w.left);
-                        if (GATE) store_some((T*)p.dgate + t * p.ld_dgate + w.channel, dz, w.left);
+                        w.store((T*)p.dx + t * p.ld_dx + w.channel, dx);
+                        w.store((T*)p.ddt + t * p.ld_ddt + w.channel, ddt);
+                        if (GATE) w.store((T*)p.dgate + t * p.ld_dgate + w.channel, dz);
                     }
                 }
                 held += TILE;
                 if (held >= 256) flush();
+                now = next;
+                frames = TILE;
             }
             if (MODE == 0) {
                 if (p.dstate_in != nullptr && u.head) scan_store_states(p.dstate_in, p, w, u.utt, g);
             } else {
-                scan_store_lanes(p.seg_state, place, w.lane, g);
+                scan_store_lanes(p.seg_state, place, w, g);
+                Pack<float, R> v;
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const float v = rows_sum(total[r], total[r]);
-                    total[r] = halves_sum(v, v);
-                }
-                if (w.row == 0) {
-                    Pack<float, R> v;
-#pragma unroll
-                    for (int r = 0; r < R; ++r) v.v[r] = total[r];
-                    store_pack(p.seg_sum + place * CH + w.col * R, v);
-                }
+                for (int r = 0; r < R; ++r) v.v[r] = quad_sum(total[r]);
+                if (w.row == 0) store_pack(p.seg_sum + place * CH + w.col * R, v);
             }
         }
         if (MODE == 0) {
@@ -662,10 +875,8 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
             const int64_t place = part * p.blocks + block;
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                float v = rows_sum(acc[(R * S + r) * 64 + w.lane], acc[(R * S + r) * 64 + w.lane]);
-                const float vs = halves_sum(v, v);
-                v = rows_sum(acc[(R * S + R + r) * 64 + w.lane], acc[(R * S + R + r) * 64 + w.lane]);
-                const float vb = halves_sum(v, v);
+                const float vs = quad_sum(acc[(R * S + r) * 64 + w.lane]);
+                const float vb = quad_sum(acc[(R * S + R + r) * 64 + w.lane]);
                 if (w.row == 0) {
                     p.part_vec[(place * 2 + 0) * CH + w.col * R + r] = vs;
                     p.part_vec[(place * 2 + 1) * CH + w.col * R + r] = vb;
@@ -673,7 +884,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
 #pragma unroll
                 for (int s = 0; s < S; ++s) dA[r][s] = acc[(r * S + s) * 64 + w.lane];
             }
-            scan_store_lanes(p.part_A, place, w.lane, dA);
+            scan_store_lanes(p.part_A, place, w, dA);
         }
     }
 }
@@ -686,7 +897,7 @@ __global__ __launch_bounds__(256) void scan_sum_parts_kernel(ScanParams p) {
     __shared__ double sum[4][64][4];
     const int block = blockIdx.x / (QUADS + 1), k = blockIdx.x % (QUADS + 1);
     const int wave = threadIdx.x >> 6;
-    const ScanLane<R, S> w(p, block);
+    const ScanLane<R, S, false> w(p, block);
     double v[4] = {0.0, 0.0, 0.0, 0.0};
     for (int64_t part = wave; part < p.parts; part += 4) {
         const int64_t place = part * p.blocks + block;
@@ -777,8 +988,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams p, float* sta
             }
             store_some(h + n0, v, left);
         }
-        y += dpp_mov<0xB1>(y);       // quad_perm [1,0,3,2]
-        y += dpp_mov<0x4E>(y);       // quad_perm [2,3,0,1]
+        y = quad_sum(y);
         if (p.skip != nullptr) y = fmaf(p.skip[c], x, y);
         if (p.gate != nullptr) {
             const float z = (float)((const T*)p.gate)[row * p.ld_gate + c];
@@ -802,7 +1012,7 @@ int scan_forward_launch(const ScanParams& p, hipStream_t st) {
     if (p.segment != 0) {
         scan_forward_kernel<T, R, S, GATE, 1><<<scan_grid(p.units * across), 64 * kScanWaves, 0, st>>>(p);
         SRX_HIP(hipGetLastError());
-        scan_join_kernel<R, S, false><<<scan_grid(p.utts * p.blocks), 64, 0, st>>>(p);
+        scan_join_kernel<R, S, false><<<scan_grid(p.utts * p.blocks * (R * S / 4)), 64 * kJoinWaves, 0, st>>>(p);
         SRX_HIP(hipGetLastError());
     }
     scan_forward_kernel<T, R, S, GATE, 0><<<scan_grid(p.units * across), 64 * kScanWaves, 0, st>>>(p);
@@ -812,18 +1022,19 @@ int scan_forward_launch(const ScanParams& p, hipStream_t st) {
 
 template <typename T, int R, int S, bool GATE>
 int scan_backward_launch(const ScanParams& q, hipStream_t st) {
+    constexpr int SUB = R * S <= 8 ? 8 : 4;              // (what the registers of two waves per SIMD hold)
     ScanParams p = q;
     const int64_t across = (p.blocks + kScanWaves - 1) / kScanWaves;
     if (p.segment != 0) {
         const int64_t parts = p.parts;
         p.parts = p.units;
-        scan_backward_kernel<T, R, S, GATE, 1><<<scan_grid(p.units * across), 64 * kScanWaves, 0, st>>>(p);
+        scan_backward_kernel<T, R, S, GATE, 1, SUB><<<scan_grid(p.units * across), 64 * kScanWaves, 0, st>>>(p);
         SRX_HIP(hipGetLastError());
-        scan_join_kernel<R, S, true><<<scan_grid(p.utts * p.blocks), 64, 0, st>>>(p);
+        scan_join_kernel<R, S, true><<<scan_grid(p.utts * p.blocks * (R * S / 4)), 64 * kJoinWaves, 0, st>>>(p);
         SRX_HIP(hipGetLastError());
         p.parts = parts;
     }
-    scan_backward_kernel<T, R, S, GATE, 0><<<scan_grid(p.parts * across), 64 * kScanWaves, 0, st>>>(p);
+    scan_backward_kernel<T, R, S, GATE, 0, SUB><<<scan_grid(p.parts * across), 64 * kScanWaves, 0, st>>>(p);
     SRX_HIP(hipGetLastError());
     scan_sum_parts_kernel<R, S><<<(unsigned)(p.blocks * (R * S / 4 + 1)), 256, 0, st>>>(p);
     SRX_HIP(hipGetLastError());
@@ -835,17 +1046,22 @@ int scan_backward_launch(const ScanParams& q, hipStream_t st) {
     return SRX_OK;
 }
 
+// The shapes of a wave that there are: 16 R channels, 4 S states (p.wide = R, see ssm_scan.hip).
 template <typename T, bool GATE>
 int scan_dispatch(const ScanParams& p, bool backward, hipStream_t st) {
 #define SRX_SCAN_CASE(R, S)                                                                   \
-    if (p.states <= 4 * S)                                                                    \
+    if (p.states <= 4 * S && p.wide == R)                                                     \
         return backward ? scan_backward_launch<T, R, S, GATE>(p, st) : scan_forward_launch<T, R, S, GATE>(p, st);
     SRX_SCAN_CASE(4, 1)
     SRX_SCAN_CASE(4, 2)
     SRX_SCAN_CASE(4, 4)
+    SRX_SCAN_CASE(2, 4)
+    SRX_SCAN_CASE(1, 4)
     SRX_SCAN_CASE(2, 8)
+    SRX_SCAN_CASE(1, 8)
     SRX_SCAN_CASE(1, 16)
 #undef SRX_SCAN_CASE
+    srx_set_error("selective scan: no kernel for %d states, %d channels a lane", p.states, p.wide);
     return SRX_EUNSUPPORTED;
 }
 

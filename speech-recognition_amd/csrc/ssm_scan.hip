@@ -4,8 +4,7 @@
 
 namespace {
 
-// Channels of a wave's block: 16 R, by the number of states (see scan_dispatch).
-int block_channels(int states) { return states <= 16 ? 64 : states <= 32 ? 32 : 16; }
+// States of a wave: 4 S.
 int block_states(int states) { return states <= 4 ? 4 : states <= 8 ? 8 : states <= 16 ? 16 : states <= 32 ? 32 : 64; }
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -33,8 +32,7 @@ int check_inputs(const srx_scan_t* s, const srx_scan_inputs_t* in, int dtype, in
     return SRX_OK;
 }
 
-// The smallest pitches that a caller may pass keep every offset far below 2^63.
-ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, int64_t frames) {
+ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, int64_t frames, bool train) {
     ScanParams p;
     memset(&p, 0, sizeof(p));
     p.A = s->A;
@@ -45,18 +43,25 @@ ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, i
     p.states = s->n_states;
     p.groups = s->n_groups;
     p.per_group = s->n_channels / s->n_groups;
-    const int ch = block_channels(s->n_states);
-    p.group_blocks = (p.per_group + ch - 1) / ch;
-    p.blocks = p.group_blocks * s->n_groups;
     p.utts = utts;
     p.frames = frames;
-    // Whole utterances where they alone give every SIMD two waves (a SIMD with a single wave issues at
-    // half its rate); else pieces, whose states are computed twice.
-    const int64_t wanted = (int64_t)h->n_cu * 4 * 2;
+    const int64_t simds = (int64_t)h->n_cu * 4;
+    auto blocks_of = [&](int wide) { return (int64_t)s->n_groups * ((p.per_group + 16 * wide - 1) / (16 * wide)); };
+    // Channels of a lane: as many as leave every SIMD several waves (a frame's work beside the exponentials is
+    // smaller for wide lanes); the registers of 32 and 64 states leave room for fewer.
+    const int most = s->n_states <= 16 ? 4 : s->n_states <= 32 ? 2 : 1;
+    const int least = s->n_states <= 8 ? 4 : 1;
+    p.wide = most;
+    if (train && s->n_states > 8 && s->n_states <= 16) p.wide = 2;
+    while (p.wide > least && utts * blocks_of(p.wide) < 4 * simds) p.wide /= 2;
+    p.group_blocks = (p.per_group + 16 * p.wide - 1) / (16 * p.wide);
+    p.blocks = p.group_blocks * s->n_groups;
+    // Whole utterances where they alone give every SIMD a wave; else pieces, whose states are computed twice.
     p.segment = 0;
     p.units = utts;
-    if (utts > 0 && utts * p.blocks < wanted) {
-        const int64_t segment = round_up(frames * p.blocks / (2 * wanted) > 64 ? frames * p.blocks / (2 * wanted) : 64, 16);
+    if (utts > 0 && utts * p.blocks < simds) {
+        const int64_t even = frames * p.blocks / (4 * simds);
+        const int64_t segment = round_up(even > 64 ? even : 64, 16);
         if (frames / utts > 2 * segment) {
             p.segment = segment;
             p.units = frames / segment + utts;
@@ -64,8 +69,8 @@ ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, i
     }
     // backward: a wave sums the parameters' gradients over all its units
     p.parts = p.units;
-    const int64_t most = 4 * wanted / p.blocks + 1;
-    if (p.segment == 0 && p.parts > most) p.parts = most;
+    const int64_t enough = 8 * simds / p.blocks + 1;
+    if (p.segment == 0 && p.parts > enough) p.parts = enough;
     if (p.parts < 1) p.parts = 1;
     return p;
 }
@@ -83,7 +88,7 @@ struct Carver {
 
 int64_t carve(ScanParams& p, bool backward, void* workspace) {
     Carver c{(char*)workspace};
-    const int64_t ch = block_channels(p.states), ns = block_states(p.states);
+    const int64_t ch = 16 * p.wide, ns = block_states(p.states);
     if (p.segment != 0) {
         p.seg_state = c.floats(p.units * p.blocks * ch * ns);
         p.seg_sum = c.floats(p.units * p.blocks * ch);
@@ -120,8 +125,14 @@ void take_inputs(ScanParams& p, const srx_scan_inputs_t* in) {
 int64_t workspace_bytes_for(srx_handle_t h, const srx_scan_t* s, int64_t utts, int64_t frames, bool backward,
                             const char* who) {
     if (check_scan(h, s, utts, frames, who)) return -1;
-    ScanParams p = params_for(h, s, utts, frames);
-    return carve(p, backward, nullptr);
+    if (backward) {
+        ScanParams p = params_for(h, s, utts, frames, true);
+        return carve(p, true, nullptr);
+    }
+    // (a pass that saves its states may cut the channels differently)
+    ScanParams p = params_for(h, s, utts, frames, false), q = params_for(h, s, utts, frames, true);
+    const int64_t a = carve(p, false, nullptr), b = carve(q, false, nullptr);
+    return a > b ? a : b;
 }
 
 }  // namespace
@@ -134,7 +145,7 @@ int64_t srx_selective_scan_saved(const srx_scan_t* s, int64_t n_utts, int64_t n_
         srx_set_error("srx_selective_scan_saved: Shape mismatch");
         return -1;
     }
-    const int64_t ch = block_channels(s->n_states), per = s->n_channels / s->n_groups;
+    const int64_t ch = 64, per = s->n_channels / s->n_groups;      // (room for every way to cut the channels)
     return (n_frames / kScanSaveEvery + n_utts) * ((per + ch - 1) / ch * s->n_groups) * ch * block_states(s->n_states);
 }
 
@@ -159,7 +170,7 @@ int srx_selective_scan(srx_handle_t h, const srx_scan_t* s, const srx_scan_input
     SRX_REQUIRE(utt_offsets != nullptr, "%s: NULL utterance offsets", who);
     SRX_REQUIRE(n_frames == 0 || y != nullptr, "%s: NULL y", who);
     SRX_REQUIRE(n_frames == 0 || ld_y >= s->n_channels, "%s: a row pitch is smaller than its row", who);
-    ScanParams p = params_for(h, s, n_utts, n_frames);
+    ScanParams p = params_for(h, s, n_utts, n_frames, saved != nullptr);
     const int64_t need = carve(p, false, workspace);
     SRX_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need),
                 "%s: workspace of %lld bytes, %lld are needed", who, (long long)workspace_bytes, (long long)need);
@@ -184,7 +195,7 @@ int srx_selective_scan_step(srx_handle_t h, const srx_scan_t* s, const srx_scan_
     if (n_rows == 0) return SRX_OK;
     SRX_REQUIRE(state != nullptr && y != nullptr, "%s: NULL state or y", who);
     SRX_REQUIRE(ld_y >= s->n_channels, "%s: a row pitch is smaller than its row", who);
-    ScanParams p = params_for(h, s, n_rows, n_rows);
+    ScanParams p = params_for(h, s, n_rows, n_rows, false);
     take_inputs(p, in);
     p.y = y;
     p.ld_y = ld_y;
@@ -220,7 +231,7 @@ int srx_selective_scan_backward(srx_handle_t h, const srx_scan_t* s, const srx_s
                         grads->ld_dC >= bc && (in->gate == nullptr || grads->ld_dgate >= c),
                     "%s: a row pitch is smaller than its row", who);
     }
-    ScanParams p = params_for(h, s, n_utts, n_frames);
+    ScanParams p = params_for(h, s, n_utts, n_frames, true);
     const int64_t need = carve(p, true, workspace);
     SRX_REQUIRE(workspace != nullptr && workspace_bytes >= need,
                 "%s: workspace of %lld bytes, %lld are needed", who, (long long)workspace_bytes, (long long)need);
