@@ -419,7 +419,8 @@ typedef struct {
     const float* dt_bias;   /* [n_channels] or NULL */
 } srx_scan_t;
 /* Inputs of the scan, one row per frame: n_channels values of x, dt and gate (NULL: no gate), n_groups x
- * n_states of B and C. */
+ * n_states of B and C.  Four rows of them (16 of B and C) must lie
+ * within 2^32 bytes: pitches up to about 2^30 (2^28) bytes. */
 typedef struct {
     const void *x, *dt, *B, *C, *gate;
     int64_t ld_x, ld_dt, ld_B, ld_C, ld_gate;

@@ -27,6 +27,29 @@ template <int V, typename T>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
     __builtin_memcpy((void*)p, &v.v, V * sizeof(T));
 }
+// The same at a scalar global address plus a 32-bit offset of the lane's own: one scalar register pair and one
+// vector register, instead of a 64-bit address in vector registers.  (The scalar part is hidden from the optimiser, which
+// would add the two up.)
+typedef __attribute__((address_space(1))) char GlobalChar;
+__device__ __forceinline__ GlobalChar* global_at(GlobalChar* base, unsigned off) {
+    asm("" : "+s"(base));
+    asm("" : "+v"(off));
+    return base + off;
+}
+template <int V, typename T>
+__device__ __forceinline__ Pack<T, V> load_global(GlobalChar* base, unsigned off) {
+    typedef typename Pack<T, V>::Vec Vec;
+    typedef Vec Loose __attribute__((aligned(sizeof(T))));
+    Pack<T, V> r;
+    r.v = *(__attribute__((address_space(1))) const Loose*)global_at(base, off);
+    return r;
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_global(GlobalChar* base, unsigned off, const Pack<T, V>& v) {
+    typedef typename Pack<T, V>::Vec Vec;
+    typedef Vec Loose __attribute__((aligned(sizeof(T))));
+    *(__attribute__((address_space(1))) Loose*)global_at(base, off) = v.v;
+}
 // The first `n` (<= V) of V neighbouring elements, zeros behind them.
 template <int V, typename T>
 __device__ __forceinline__ Pack<T, V> load_some(const T* p, int n) {
@@ -60,22 +83,37 @@ __device__ __forceinline__ float sigmoid_f32(float x) {
     // (the exponential overflows to infinity for x below -88, the quotient is then zero)
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x));
 }
-// ln(1 + e^x) = max(x, 0) + log1p(e^-|x|); log1p(e) = 2 artanh(e / (2 + e)) by its power series,
-// whose argument is at most 1/3: seven terms leave 1.5e-8 of the value, and small values keep
-// their relative accuracy (steps of 0.001 and less are ordinary).
+// ln(1 + e^x) = max(x, 0) + log1p(e^-|x|).  log1p(e): the logarithm of u = 1 + e, plus what the rounding
+// of that sum dropped, which for a small e is most of its relative accuracy (steps of 0.001 and less
+// are ordinary); its derivative 1 / u is taken as 1, as the dropped part is below 2^-24.  The exponential is
+// off by |x| 2^-24 of itself, as much as x is when it is itself a rounded sum.  A NaN comes through the exponential.
 __device__ __forceinline__ float softplus_f32(float x) {
-    const float e = exp_f32(-fabsf(x));
-    const float s = e * __builtin_amdgcn_rcpf(2.0f + e);
-    const float q = s * s;
-    float p = fmaf(q, 1.0f / 13.0f, 1.0f / 11.0f);
-    p = fmaf(p, q, 1.0f / 9.0f);
-    p = fmaf(p, q, 1.0f / 7.0f);
-    p = fmaf(p, q, 1.0f / 5.0f);
-    p = fmaf(p, q, 1.0f / 3.0f);
-    p = fmaf(p * q, 2.0f * s, 2.0f * s);
-    // (not fmaxf: a NaN has to come through)
-    return (x > 0.0f ? x : (x == x ? 0.0f : x)) + p;
+    const float e = __builtin_amdgcn_exp2f(-1.44269504088896341f * fabsf(x));
+    const float u = 1.0f + e;
+    return fmaxf(x, 0.0f) + fmaf(__builtin_amdgcn_logf(u), 0.693147180559945309f, e - (u - 1.0f));
 }
+
+// Makes the wave wait here for the loads into v, and not later, behind stores that follow: loads and stores
+// complete in order, and a wait for a load behind a store that a branch may have skipped waits for the store too.
+template <typename T, int V>
+__device__ __forceinline__ void arrive(Pack<T, V>& v) {
+    constexpr int WORDS = (sizeof(T) * V + 3) / 4;
+    if constexpr (sizeof(T) * V == 2) {
+        unsigned short u;
+        __builtin_memcpy(&u, &v.v, 2);
+        unsigned w = u;
+        asm volatile("" : "+v"(w));
+        u = (unsigned short)w;
+        __builtin_memcpy(&v.v, &u, 2);
+    } else {
+        unsigned w[WORDS];
+        __builtin_memcpy(w, &v.v, WORDS * 4);
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[i]));
+        __builtin_memcpy(&v.v, w, WORDS * 4);
+    }
+}
+__device__ __forceinline__ void arrive(float& v) { asm volatile("" : "+v"(v)); }
 
 // Orders the LDS traffic of one wave: its lanes read what other lanes of it wrote.  The hardware
 // runs a wave's LDS instructions in order; this keeps the compiler from moving them.

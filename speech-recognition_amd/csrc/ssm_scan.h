@@ -101,11 +101,46 @@ __device__ __forceinline__ bool scan_unit(const ScanParams& p, int64_t unit, Sca
     return true;
 }
 
+// A value that is the same in all lanes, in scalar registers.
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v);
+    const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)((uint64_t)v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ void uniform_unit(ScanUnit& u) {
+    u.utt = uniform64(u.utt);
+    u.begin = uniform64(u.begin);
+    u.first = uniform64(u.first);
+    u.last = uniform64(u.last);
+}
+
+// The rows of one matrix as a wave walks over them: a scalar address that moves with the frames and a
+// 32-bit offset of the lane's own (its row among the first `frames` of a tile, its channel), so that a walk over
+// eight matrices costs eight vector registers.  (The entry points refuse pitches that offset cannot reach.)
+template <typename T>
+struct ScanRows {
+    GlobalChar* at;          // frame 0 of the tile
+    int64_t pitch;           // bytes
+    unsigned off;
+    __device__ __forceinline__ ScanRows() {}
+    __device__ __forceinline__ ScanRows(const void* base, int64_t ld, int64_t frame, int row, int column) {
+        pitch = ld * (int64_t)sizeof(T);
+        at = (GlobalChar*)const_cast<void*>(base) + frame * pitch;
+        off = (unsigned)row * (unsigned)pitch + (unsigned)column * (unsigned)sizeof(T);
+    }
+    template <int V>
+    __device__ __forceinline__ Pack<T, V> load(int more) const { return load_global<V, T>(at + more * pitch, off); }
+    template <int V>
+    __device__ __forceinline__ void store(int more, const Pack<T, V>& v) const { store_global<V, T>(at + more * pitch, off, v); }
+    __device__ __forceinline__ void move(int frames) { at += frames * pitch; }
+};
+
 // Channels of a wave's block, and where they are.  QUADS false: the four rows of 16 lanes hold the four groups of
 // states, lane 16 row + col; true: four neighbouring lanes do, lane 4 col + row.
 template <int R, int S, bool QUADS>
 struct ScanLane {
     static constexpr int kChannels = 16 * R, kStates = 4 * S;
+    static_assert(R * S % 4 == 0, "states move in fours");
     int lane, row, col;
     int group, channel, left;    // first channel of this lane, how many of its R exist
     int end;                     // the group's last channel
@@ -113,6 +148,7 @@ struct ScanLane {
     bool full;                   // the block has all its channels (the same for the whole wave)
     __device__ __forceinline__ ScanLane(const ScanParams& p, int block) {
         lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));       // (or what follows from it would wait in registers from task to task)
         row = QUADS ? lane & 3 : lane >> 4;
         col = QUADS ? lane >> 2 : lane & 15;
         group = block / p.group_blocks;
@@ -123,37 +159,44 @@ struct ScanLane {
         state = row * S;
         full = first + kChannels <= p.per_group;
     }
-    // R neighbouring values of a frame's row, `at` the address of this lane's first.  Without them all the last one
-    // stands in for those that do not exist: no branch, nothing behind the row is touched.
+    // R neighbouring values of frame 4 i + row, or of frame `last` where that is behind it.  A whole block's are one
+    // access without a branch; elsewhere the group's last channel stands in for those that do not exist.
     template <typename T>
-    __device__ __forceinline__ Pack<T, R> load(const T* at, bool fast) const {
-        if (fast) return load_pack<R>(at);
+    __device__ __forceinline__ Pack<T, R> load_any(const ScanRows<T>& rows, int i, int last) const {
+        int t = min(4 * i + row, last), c = channel;
+        asm volatile("" : "+v"(t), "+v"(c));             // (nothing of this is worth a register in the loop)
+        const T* at = (const T*)(rows.at + t * rows.pitch);
         Pack<T, R> v;
 #pragma unroll
-        for (int r = 0; r < R; ++r) v.v[r] = at[min(channel + r, end) - channel];
+        for (int r = 0; r < R; ++r) v.v[r] = at[min(c + r, end)];
+        __builtin_amdgcn_sched_barrier(0);               // (one row's addresses at a time)
         return v;
     }
     template <typename T>
-    __device__ __forceinline__ void store(T* at, const Pack<T, R>& v) const {
+    __device__ __forceinline__ void store(const ScanRows<T>& rows, int i, const Pack<T, R>& v) const {
         if (full) {
-            store_pack(at, v);
+            rows.template store<R>(4 * i, v);
             return;
         }
+        T* at = (T*)global_at(rows.at + 4 * i * rows.pitch, rows.off);
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (r < left) at[r] = v.v[r];
     }
 };
-// S states of a frame's B or C from state s0 on, zeros for those that do not exist.
+// S states of frame t of a tile's B or C from state s0 on, zeros for those that do not exist.
 template <int S, typename T>
-__device__ __forceinline__ Pack<T, S> scan_load_bc(const T* at, int s0, int states, bool fast) {
-    if (fast) return load_pack<S>(at);
+__device__ __forceinline__ Pack<T, S> scan_load_bc(const ScanRows<T>& rows, int t, int last, int group, int s0, int states) {
+    t = min(t, last);
+    asm volatile("" : "+v"(t), "+v"(s0));
+    const T* at = (const T*)(rows.at + t * rows.pitch) + (int64_t)group * states;
     Pack<T, S> v;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        const T x = at[min(s0 + s, states - 1) - s0];
+        const T x = at[min(s0 + s, states - 1)];
         v.v[s] = s0 + s < states ? x : (T)0.0f;
     }
+    __builtin_amdgcn_sched_barrier(0);
     return v;
 }
 
@@ -222,59 +265,63 @@ template <typename T, int R, int S, bool GATE, bool WITH_Y>
 struct ScanTileRaw {
     Pack<T, R> x[4], dt[4], z[4];
     Pack<T, S> b, c;
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            arrive(x[i]);
+            arrive(dt[i]);
+            if (GATE && WITH_Y) arrive(z[i]);
+        }
+        arrive(b);
+        if (WITH_Y) arrive(c);
+    }
 };
 template <typename T, int R, int S, bool GATE, bool WITH_Y>
 struct ScanTileReader {
-    const T *x, *dt, *z, *b, *c;
-    int64_t ld_x, ld_dt, ld_z, ld_b, ld_c;
+    ScanRows<T> x, dt, z, b, c;
     bool all_states;
     __device__ __forceinline__ ScanTileReader(const ScanParams& p, const ScanLane<R, S, false>& w, int64_t first) {
-        ld_x = p.ld_x;
-        ld_dt = p.ld_dt;
-        ld_z = p.ld_gate;
-        ld_b = p.ld_B;
-        ld_c = p.ld_C;
-        const int64_t t = first + w.row, tb = first + (w.lane >> 2);
-        const int64_t s0 = (int64_t)w.group * p.states + (w.lane & 3) * S;
-        x = (const T*)p.x + t * ld_x + w.channel;
-        dt = (const T*)p.dt + t * ld_dt + w.channel;
-        z = GATE && WITH_Y ? (const T*)p.gate + t * ld_z + w.channel : nullptr;
-        b = (const T*)p.B + tb * ld_b + s0;
-        c = WITH_Y ? (const T*)p.C + tb * ld_c + s0 : nullptr;
+        const int s0 = w.group * p.states + (w.lane & 3) * S;
+        x = ScanRows<T>(p.x, p.ld_x, first, w.row, w.channel);
+        dt = ScanRows<T>(p.dt, p.ld_dt, first, w.row, w.channel);
+        if (GATE && WITH_Y) z = ScanRows<T>(p.gate, p.ld_gate, first, w.row, w.channel);
+        b = ScanRows<T>(p.B, p.ld_B, first, w.lane >> 2, s0);
+        if (WITH_Y) c = ScanRows<T>(p.C, p.ld_C, first, w.lane >> 2, s0);
         all_states = p.states == 4 * S;
     }
     // The next `frames` frames (at least one): a whole tile without a branch, a shorter one with its last frame in
     // place of those behind it, which are not used.
     __device__ __forceinline__ void next(const ScanParams& p, const ScanLane<R, S, false>& w, int64_t frames,
                                          ScanTileRaw<T, R, S, GATE, WITH_Y>& to) {
-        const int s0 = (w.lane & 3) * S;
-        if (frames >= kScanTile && w.full) {
+        const int last = (int)min(frames, (int64_t)kScanTile) - 1;
+        if (last == kScanTile - 1 && w.full) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                to.x[i] = load_pack<R>(x + 4 * i * ld_x);
-                to.dt[i] = load_pack<R>(dt + 4 * i * ld_dt);
-                if (GATE && WITH_Y) to.z[i] = load_pack<R>(z + 4 * i * ld_z);
+                to.x[i] = x.template load<R>(4 * i);
+                to.dt[i] = dt.template load<R>(4 * i);
+                if (GATE && WITH_Y) to.z[i] = z.template load<R>(4 * i);
             }
-            to.b = scan_load_bc<S>(b, s0, p.states, all_states);
-            if (WITH_Y) to.c = scan_load_bc<S>(c, s0, p.states, all_states);
         } else {
-            const int last = (int)min(frames, (int64_t)kScanTile) - 1;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int64_t t = min(4 * i + w.row, last) - w.row;
-                to.x[i] = w.load(x + t * ld_x, w.full);
-                to.dt[i] = w.load(dt + t * ld_dt, w.full);
-                if (GATE && WITH_Y) to.z[i] = w.load(z + t * ld_z, w.full);
+                to.x[i] = w.load_any(x, i, last);
+                to.dt[i] = w.load_any(dt, i, last);
+                if (GATE && WITH_Y) to.z[i] = w.load_any(z, i, last);
             }
-            const int64_t t = min(w.lane >> 2, last) - (w.lane >> 2);
-            to.b = scan_load_bc<S>(b + t * ld_b, s0, p.states, all_states);
-            if (WITH_Y) to.c = scan_load_bc<S>(c + t * ld_c, s0, p.states, all_states);
         }
-        x += kScanTile * ld_x;
-        dt += kScanTile * ld_dt;
-        if (GATE && WITH_Y) z += kScanTile * ld_z;
-        b += kScanTile * ld_b;
-        if (WITH_Y) c += kScanTile * ld_c;
+        if (last == kScanTile - 1 && all_states) {
+            to.b = b.template load<S>(0);
+            if (WITH_Y) to.c = c.template load<S>(0);
+        } else {
+            const int s0 = (w.lane & 3) * S;
+            to.b = scan_load_bc<S>(b, w.lane >> 2, last, w.group, s0, p.states);
+            if (WITH_Y) to.c = scan_load_bc<S>(c, w.lane >> 2, last, w.group, s0, p.states);
+        }
+        x.move(kScanTile);
+        dt.move(kScanTile);
+        if (GATE && WITH_Y) z.move(kScanTile);
+        b.move(kScanTile);
+        if (WITH_Y) c.move(kScanTile);
     }
 };
 
@@ -310,6 +357,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
         const int block = (int)(task - unit * across) * kScanWaves + wave;
         ScanUnit u;
         if (block >= p.blocks || !scan_unit(p, unit, u)) continue;
+        uniform_unit(u);
         const ScanLane<R, S, false> w(p, block);
         float A2[R][S], h[R][S], bias[R], skip[R], total[R];
         scan_load_A(p, w, A2);
@@ -332,7 +380,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
         const int64_t frames = u.last - u.first;
         ScanTileReader<T, R, S, GATE, MODE == 0> reader(p, w, u.first);
         ScanTileRaw<T, R, S, GATE, MODE == 0> now, next;
-        T* y = (T*)p.y + (u.first + w.row) * p.ld_y + w.channel;
+        ScanRows<T> y(p.y, p.ld_y, u.first, w.row, w.channel);
         float* saved = nullptr;
         if (MODE == 0 && p.saved != nullptr)
             saved = p.saved + (scan_slot(u, u.first) * p.blocks + block) * (R * S * 64);
@@ -343,16 +391,23 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
             wave_lds_fence();                            // the last tile has been read
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool live = 4 * i + w.row < here;
                 Pack<float, R> d, du;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     const float raw = (float)now.dt[i].v[r] + bias[r];
-                    const float step = p.softplus ? softplus_f32(raw) : raw;
-                    d.v[r] = live ? step : 0.0f;         // a frame behind the last one changes nothing
-                    du.v[r] = live ? step * (float)now.x[i].v[r] : 0.0f;
-                    if (MODE == 1) total[r] += d.v[r];
+                    d.v[r] = p.softplus ? softplus_f32(raw) : raw;
+                    du.v[r] = d.v[r] * (float)now.x[i].v[r];
                 }
+                if (here < TILE) {                       // a frame behind the last one changes nothing
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        d.v[r] = 4 * i + w.row < here ? d.v[r] : 0.0f;
+                        du.v[r] = 4 * i + w.row < here ? du.v[r] : 0.0f;
+                    }
+                }
+                if (MODE == 1)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) total[r] += d.v[r];
                 store_pack(sD + (4 * i + w.row) * CH + w.col * R, d);
                 store_pack(sU + (4 * i + w.row) * CH + w.col * R, du);
             }
@@ -369,6 +424,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
             wave_lds_fence();
             ScanFrame<R, S> f;
             f.template load<true, MODE == 0>(w, 0, sD, sU, nullptr, sB, sC);
+            Pack<T, R> out[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (MODE == 0 && i % 2 == 0 && saved != nullptr && 4 * i < here) {
@@ -395,7 +451,6 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
                 }
                 if (MODE == 0) {
                     // the four rows' shares added up; row g is left with frame 4 i + g
-                    Pack<T, R> out;
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
                         float v = rows_sum(halves_sum(part[0][r], part[2][r]), halves_sum(part[1][r], part[3][r]));
@@ -404,13 +459,18 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
                             const float z = (float)now.z[i].v[r];
                             v *= z * sigmoid_f32(z);
                         }
-                        out.v[r] = (T)v;                 // the one rounding to the output's type
+                        out[i].v[r] = (T)v;              // the one rounding to the output's type
                     }
-                    if (4 * i + w.row < here) w.store(y, out);
-                    y += 4 * p.ld_y;
                 }
             }
             now = next;
+            now.arrived();
+            if (MODE == 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (4 * i + w.row < here) w.store(y, i, out[i]);
+                y.move(TILE);
+            }
         }
         if (MODE == 0) {
             if (p.state_out != nullptr && u.tail) scan_store_states(p.state_out, p, w, u.utt, h);
@@ -522,59 +582,88 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanParams p
 template <typename T, int R, int S, bool GATE>
 struct ScanOctetRaw {
     Pack<T, R> x[2], dt[2], z[2], dy[2];
-    Pack<T, S> bc;               // lanes 0 .. 31: B, lanes 32 .. 63: C
+    Pack<T, S> b, c;             // (lanes 32 .. 63 the same as lanes 0 .. 31)
+    // x, dt, z and dy are needed at both ends of an octet's work; in between they lie in LDS.
+    static constexpr int kStash = (int)sizeof(Pack<T, R>) < 4 ? 4 : (int)sizeof(Pack<T, R>);       // bytes a lane
+    __device__ __forceinline__ void put(char* at) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            __builtin_memcpy(at + (0 + i) * 64 * kStash, &x[i].v, sizeof(x[i].v));
+            __builtin_memcpy(at + (2 + i) * 64 * kStash, &dt[i].v, sizeof(x[i].v));
+            __builtin_memcpy(at + (4 + i) * 64 * kStash, &dy[i].v, sizeof(x[i].v));
+            if (GATE) __builtin_memcpy(at + (6 + i) * 64 * kStash, &z[i].v, sizeof(x[i].v));
+        }
+    }
+    __device__ __forceinline__ void get(const char* at) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            __builtin_memcpy(&x[i].v, at + (0 + i) * 64 * kStash, sizeof(x[i].v));
+            __builtin_memcpy(&dt[i].v, at + (2 + i) * 64 * kStash, sizeof(x[i].v));
+            __builtin_memcpy(&dy[i].v, at + (4 + i) * 64 * kStash, sizeof(x[i].v));
+            if (GATE) __builtin_memcpy(&z[i].v, at + (6 + i) * 64 * kStash, sizeof(x[i].v));
+        }
+    }
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            arrive(x[i]);
+            arrive(dt[i]);
+            if (GATE) arrive(z[i]);
+            arrive(dy[i]);
+        }
+        arrive(b);
+        arrive(c);
+    }
 };
 template <typename T, int R, int S, bool GATE>
 struct ScanOctetReader {
-    const T *x, *dt, *z, *dy, *bc;
-    int64_t ld_x, ld_dt, ld_z, ld_dy, ld_bc;
+    ScanRows<T> x, dt, z, dy, b, c;
     bool all_states;
     // `first`: the first frame of the octet that is read first; later ones lie before it
     __device__ __forceinline__ ScanOctetReader(const ScanParams& p, const ScanLane<R, S, true>& w, int64_t first) {
-        ld_x = p.ld_x;
-        ld_dt = p.ld_dt;
-        ld_z = p.ld_gate;
-        ld_dy = p.ld_dy;
-        ld_bc = w.lane < 32 ? p.ld_B : p.ld_C;
-        const int64_t t = first + w.row;
-        x = (const T*)p.x + t * ld_x + w.channel;
-        dt = (const T*)p.dt + t * ld_dt + w.channel;
-        z = GATE ? (const T*)p.gate + t * ld_z + w.channel : nullptr;
-        dy = (const T*)p.dy + t * ld_dy + w.channel;
-        bc = (const T*)(w.lane < 32 ? p.B : p.C) + (first + ((w.lane & 31) >> 2)) * ld_bc + (int64_t)w.group * p.states +
-             (w.lane & 3) * S;
+        const int s0 = w.group * p.states + (w.lane & 3) * S, t = (w.lane & 31) >> 2;
+        x = ScanRows<T>(p.x, p.ld_x, first, w.row, w.channel);
+        dt = ScanRows<T>(p.dt, p.ld_dt, first, w.row, w.channel);
+        if (GATE) z = ScanRows<T>(p.gate, p.ld_gate, first, w.row, w.channel);
+        dy = ScanRows<T>(p.dy, p.ld_dy, first, w.row, w.channel);
+        b = ScanRows<T>(p.B, p.ld_B, first, t, s0);
+        c = ScanRows<T>(p.C, p.ld_C, first, t, s0);
         all_states = p.states == 4 * S;
     }
     __device__ __forceinline__ void next(const ScanParams& p, const ScanLane<R, S, true>& w, int frames,
                                          ScanOctetRaw<T, R, S, GATE>& to) {
-        const int s0 = (w.lane & 3) * S;
-        if (frames >= kScanSaveEvery && w.full) {
+        const int last = frames - 1;
+        if (last == kScanSaveEvery - 1 && w.full) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                to.x[i] = load_pack<R>(x + 4 * i * ld_x);
-                to.dt[i] = load_pack<R>(dt + 4 * i * ld_dt);
-                if (GATE) to.z[i] = load_pack<R>(z + 4 * i * ld_z);
-                to.dy[i] = load_pack<R>(dy + 4 * i * ld_dy);
+                to.x[i] = x.template load<R>(4 * i);
+                to.dt[i] = dt.template load<R>(4 * i);
+                if (GATE) to.z[i] = z.template load<R>(4 * i);
+                to.dy[i] = dy.template load<R>(4 * i);
             }
-            to.bc = scan_load_bc<S>(bc, s0, p.states, all_states);
         } else {
-            const int last = min(frames, kScanSaveEvery) - 1;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int64_t t = min(4 * i + w.row, last) - w.row;
-                to.x[i] = w.load(x + t * ld_x, w.full);
-                to.dt[i] = w.load(dt + t * ld_dt, w.full);
-                if (GATE) to.z[i] = w.load(z + t * ld_z, w.full);
-                to.dy[i] = w.load(dy + t * ld_dy, w.full);
+                to.x[i] = w.load_any(x, i, last);
+                to.dt[i] = w.load_any(dt, i, last);
+                if (GATE) to.z[i] = w.load_any(z, i, last);
+                to.dy[i] = w.load_any(dy, i, last);
             }
-            const int at = (w.lane & 31) >> 2;
-            to.bc = scan_load_bc<S>(bc + (int64_t)(min(at, last) - at) * ld_bc, s0, p.states, all_states);
         }
-        x -= kScanSaveEvery * ld_x;
-        dt -= kScanSaveEvery * ld_dt;
-        if (GATE) z -= kScanSaveEvery * ld_z;
-        dy -= kScanSaveEvery * ld_dy;
-        bc -= kScanSaveEvery * ld_bc;
+        if (last == kScanSaveEvery - 1 && all_states) {
+            to.b = b.template load<S>(0);
+            to.c = c.template load<S>(0);
+        } else {
+            const int s0 = (w.lane & 3) * S, t = (w.lane & 31) >> 2;
+            to.b = scan_load_bc<S>(b, t, last, w.group, s0, p.states);
+            to.c = scan_load_bc<S>(c, t, last, w.group, s0, p.states);
+        }
+        x.move(-kScanSaveEvery);
+        dt.move(-kScanSaveEvery);
+        if (GATE) z.move(-kScanSaveEvery);
+        dy.move(-kScanSaveEvery);
+        b.move(-kScanSaveEvery);
+        c.move(-kScanSaveEvery);
     }
 };
 
@@ -601,7 +690,8 @@ template <typename T, int R, int S, bool GATE, int MODE, int SUB>
 __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanParams p) {
     constexpr int CH = 16 * R, NS = 4 * S, TILE = kScanSaveEvery;
     constexpr float kLn2 = 0.693147180559945309f;
-    __shared__ __align__(16) float lds[kScanWaves][TILE * (6 * CH + 2 * NS) + (MODE == 0 ? 64 * (R * S + 2 * R) : 0)];
+    constexpr int kStash = ScanOctetRaw<T, R, S, GATE>::kStash;
+    __shared__ __align__(16) float lds[kScanWaves][TILE * (6 * CH + 4 * NS) + (MODE == 0 ? 64 * (R * S + 2 * R + 2 * kStash) : 0)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* sD = lds[wave];               // steps
     float* sU = sD + TILE * CH;          // step times x
@@ -611,7 +701,9 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
     float* oY = oD + TILE * CH;          // C h
     float* sB = oY + TILE * CH;
     float* sC = sB + TILE * NS;
-    float* acc = sC + TILE * NS;         // [R S + 2 R][64]: dA, dskip, dbias of the frames so far
+    float* oBC = sC + TILE * NS;         // [frame][B, C][state]: sums over the channels
+    float* acc = oBC + 2 * TILE * NS;    // [R S + 2 R][64]: dA, dskip, dbias of the frames so far
+    char* stash = (char*)(acc + 64 * (R * S + 2 * R)) + (threadIdx.x & 63) * kStash;
     const int across = (p.blocks + kScanWaves - 1) / kScanWaves;
     for (int64_t task = blockIdx.x; task < p.parts * across; task += gridDim.x) {
         const int64_t part = task / across;
@@ -652,6 +744,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
         for (int64_t unit = unit0; unit < unit1; ++unit) {
             ScanUnit u;
             if (!scan_unit(p, unit, u)) continue;
+            uniform_unit(u);
             const int64_t place = unit * p.blocks + block;
             float g[R][S];
             if (MODE == 0) {
@@ -669,6 +762,12 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
             const int64_t begin = u.first + (octets - 1) * TILE;           // of the last octet
             ScanOctetReader<T, R, S, GATE> reader(p, w, begin);
             ScanOctetRaw<T, R, S, GATE> now, next;
+            ScanRows<T> dx, ddt, dz;
+            if (MODE == 0) {
+                dx = ScanRows<T>(p.dx, p.ld_dx, begin, w.row, w.channel);
+                ddt = ScanRows<T>(p.ddt, p.ld_ddt, begin, w.row, w.channel);
+                if (GATE) dz = ScanRows<T>(p.dgate, p.ld_dgate, begin, w.row, w.channel);
+            }
             const float* saved = MODE == 0 ? p.saved + (scan_slot(u, begin) * p.blocks + block) * (R * S * 64) : nullptr;
             float h0[R][S];
             int frames = (int)(u.last - begin);
@@ -679,9 +778,9 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
 #pragma unroll 1
             for (int64_t o = octets - 1; o >= 0; --o) {
                 const int64_t t0 = u.first + o * TILE;
-                if (o > 0) reader.next(p, w, TILE, next);
+                float h0next[R][S];
+                if (MODE == 1 && o > 0) reader.next(p, w, TILE, next);
                 wave_lds_fence();
-                float step[2][R], dp[2][R];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const bool live = 4 * i + w.row < frames;
@@ -699,8 +798,6 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                             dv *= z * sigmoid_f32(z);
                         }
                         q.v[r] = in ? dv : 0.0f;
-                        step[i][r] = d.v[r];
-                        dp[i][r] = q.v[r];
                         if (MODE == 1) total[r] += d.v[r];
                     }
                     store_pack(sD + (4 * i + w.row) * CH + w.col * R, d);
@@ -708,12 +805,17 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                     store_pack(sP + (4 * i + w.row) * CH + w.col * R, q);
                 }
                 {
-                    Pack<float, S> v;
+                    Pack<float, S> b, c;
 #pragma unroll
-                    for (int s = 0; s < S; ++s) v.v[s] = (float)now.bc.v[s];
-                    store_pack((w.lane < 32 ? sB : sC) + (w.lane & 31) * S, v);
+                    for (int s = 0; s < S; ++s) {
+                        b.v[s] = (float)now.b.v[s];
+                        c.v[s] = (float)now.c.v[s];
+                    }
+                    store_pack(sB + (w.lane & 31) * S, b);
+                    store_pack(sC + (w.lane & 31) * S, c);
                 }
                 wave_lds_fence();
+                if (MODE == 0) now.put(stash);
                 if (MODE == 1) {
 #pragma unroll
                     for (int j = TILE - 1; j >= 0; --j) {
@@ -726,6 +828,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                                 g[r][s] = fmaf(f.q.v[r], f.c.v[s], g[r][s]) * __builtin_amdgcn_exp2f(f.d.v[r] * A2[r][s]);
                     }
                     now = next;
+                    now.arrived();
                     frames = TILE;
                     continue;
                 }
@@ -747,9 +850,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                         if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                float* to_bc = p.part_bc + ((int64_t)block * p.frames + t0) * 2 * NS + (w.lane >> 5) * NS + w.state +
-                               (S > 1 ? ((w.lane >> 4) & 1) * (S / 2) : 0);
-                const bool writes_bc = (w.lane & 12) == 0 && (S > 1 || (w.lane & 16) == 0);
+                float* to_bc = oBC + (w.lane >> 5) * NS + w.state + (S > 1 ? ((w.lane >> 4) & 1) * (S / 2) : 0);
 #pragma unroll 1
                 for (int half = TILE / SUB - 1; half >= 0; --half) {
                     const int j0 = half * SUB;
@@ -771,18 +872,11 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                             }
                         if (k % 2 == 1) __builtin_amdgcn_sched_barrier(0);
                     }
-                    // the next octet's first states are on their way while this one's gradients are computed
-                    if (half == 0 && o > 0) {
-                        saved -= (int64_t)p.blocks * (R * S * 64);
-                        scan_load_lanes(saved, 0, w, h0);
-                    }
-                    ScanFrame<R, S> f;
-                    f.template load<true, true>(w, j0 + SUB - 1, sD, sU, sP, sB, sC);
 #pragma unroll
                     for (int k = SUB - 1; k >= 0; --k) {
                         const int j = j0 + k;
-                        ScanFrame<R, S> ahead;
-                        if (k > 0) ahead.template load<true, true>(w, j - 1, sD, sU, sP, sB, sC);
+                        ScanFrame<R, S> f;
+                        f.template load<true, true>(w, j, sD, sU, sP, sB, sC);
                         float db[S], dc[S];
                         Pack<float, R> su, sd, sy;
 #pragma unroll
@@ -812,52 +906,74 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                         constexpr int HALF = S > 1 ? S / 2 : 1;
                         float sums[HALF];
                         scan_sum_channels<S>(db, dc, sums);
-                        if (writes_bc && j < frames) {
-                            Pack<float, HALF> v;
+                        Pack<float, HALF> v;
 #pragma unroll
-                            for (int s = 0; s < HALF; ++s) v.v[s] = sums[s];
-                            store_pack(to_bc + j * 2 * NS, v);
+                        for (int s = 0; s < HALF; ++s) v.v[s] = sums[s];
+                        store_pack(to_bc + j * 2 * NS, v);              // (the lanes of a row, the same values)
+                        // What the next octet needs is asked for when the last frame's registers are free.
+                        if (half == 0 && k == SUB - 1 && o > 0) {
+                            saved -= (int64_t)p.blocks * (R * S * 64);
+                            scan_load_lanes(saved, 0, w, h0next);
                         }
-                        f = ahead;
+                        if (half == 0 && k == SUB - 2 && o > 0) reader.next(p, w, TILE, next);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
                 wave_lds_fence();
+                now.get(stash);
+                const Pack<float, S> sums = load_pack<S>(oBC + w.lane * S);
+                Pack<T, R> vx[2], vt[2], vz[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int64_t t = t0 + 4 * i + w.row;
                     const bool live = 4 * i + w.row < frames;
                     const Pack<float, R> vu = load_pack<R>(oU + (4 * i + w.row) * CH + w.col * R);
                     const Pack<float, R> vd = load_pack<R>(oD + (4 * i + w.row) * CH + w.col * R);
                     Pack<float, R> vy;
                     if (GATE) vy = load_pack<R>(oY + (4 * i + w.row) * CH + w.col * R);
-                    Pack<T, R> dx, ddt, dz;
+                    const Pack<float, R> step = load_pack<R>(sD + (4 * i + w.row) * CH + w.col * R);
+                    const Pack<float, R> dp = load_pack<R>(sP + (4 * i + w.row) * CH + w.col * R);
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
                         const float x = (float)now.x[i].v[r];
-                        dx.v[r] = (T)fmaf(vu.v[r], step[i][r], dp[i][r] * skip[r]);
+                        vx[i].v[r] = (T)fmaf(vu.v[r], step.v[r], dp.v[r] * skip[r]);
                         float v = fmaf(vd.v[r], kLn2, vu.v[r] * x);
                         if (p.softplus) v *= sigmoid_f32((float)now.dt[i].v[r] + bias[r]);
-                        ddt.v[r] = (T)v;
+                        vt[i].v[r] = (T)v;
                         if (live) {
                             dbias[r] += v;
-                            dskip[r] = fmaf(dp[i][r], x, dskip[r]);
+                            dskip[r] = fmaf(dp.v[r], x, dskip[r]);
                         }
                         if (GATE) {
                             const float z = (float)now.z[i].v[r], sig = sigmoid_f32(z);
                             const float out = fmaf(skip[r], x, vy.v[r]);
-                            dz.v[r] = (T)((float)now.dy[i].v[r] * out * sig * fmaf(z, 1.0f - sig, 1.0f));
+                            vz[i].v[r] = (T)((float)now.dy[i].v[r] * out * sig * fmaf(z, 1.0f - sig, 1.0f));
                         }
-                    }
-                    if (live) {
-                        w.store((T*)p.dx + t * p.ld_dx + w.channel, dx);
-                        w.store((T*)p.ddt + t * p.ld_ddt + w.channel, ddt);
-                        if (GATE) w.store((T*)p.dgate + t * p.ld_dgate + w.channel, dz);
                     }
                 }
                 held += TILE;
                 if (held >= 256) flush();
                 now = next;
+                now.arrived();
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int s = 0; s < S; ++s) {
+                        h0[r][s] = h0next[r][s];
+                        arrive(h0[r][s]);
+                    }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (4 * i + w.row < frames) {
+                        w.store(dx, i, vx[i]);
+                        w.store(ddt, i, vt[i]);
+                        if (GATE) w.store(dz, i, vz[i]);
+                    }
+                }
+                dx.move(-TILE);
+                ddt.move(-TILE);
+                if (GATE) dz.move(-TILE);
+                if ((w.lane >> 3) < frames)
+                    store_global<S, float>((GlobalChar*)(p.part_bc + ((int64_t)block * p.frames + t0) * 2 * NS), w.lane * S * 4, sums);
                 frames = TILE;
             }
             if (MODE == 0) {
@@ -1053,11 +1169,9 @@ int scan_dispatch(const ScanParams& p, bool backward, hipStream_t st) {
     if (p.states <= 4 * S && p.wide == R)                                                     \
         return backward ? scan_backward_launch<T, R, S, GATE>(p, st) : scan_forward_launch<T, R, S, GATE>(p, st);
     SRX_SCAN_CASE(4, 1)
-    SRX_SCAN_CASE(4, 2)
-    SRX_SCAN_CASE(4, 4)
+    SRX_SCAN_CASE(2, 2)
     SRX_SCAN_CASE(2, 4)
     SRX_SCAN_CASE(1, 4)
-    SRX_SCAN_CASE(2, 8)
     SRX_SCAN_CASE(1, 8)
     SRX_SCAN_CASE(1, 16)
 #undef SRX_SCAN_CASE

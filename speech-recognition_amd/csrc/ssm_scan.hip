@@ -1,6 +1,7 @@
 // Entry points of the selective state space scan: argument checks, the choice between whole
 // utterances and pieces of them, and the division of the caller's workspace (kernels: ssm_scan.h).
 #include "ssm_scan.h"
+#include <stdlib.h>
 
 namespace {
 
@@ -20,6 +21,12 @@ int check_scan(srx_handle_t h, const srx_scan_t* s, int64_t utts, int64_t frames
     return SRX_OK;
 }
 
+// A wave reaches its rows with 32-bit offsets from the first: 4 rows of the channels' matrices, 16 of B and C.
+bool pitch_fits(int64_t ld, int64_t width, int dtype, int rows) {
+    const int64_t size = dtype == SRX_F32 ? 4 : 2;
+    return ld < ((int64_t)1 << 32) && ((rows - 1) * ld + width) * size <= 0xffffffffll;
+}
+
 int check_inputs(const srx_scan_t* s, const srx_scan_inputs_t* in, int dtype, int64_t frames, const char* who) {
     SRX_REQUIRE(frame_dtype(dtype), "%s: unknown dtype %d", who, dtype);
     SRX_REQUIRE(in != nullptr, "%s: inputs are NULL", who);
@@ -29,6 +36,9 @@ int check_inputs(const srx_scan_t* s, const srx_scan_inputs_t* in, int dtype, in
     SRX_REQUIRE(in->ld_x >= c && in->ld_dt >= c && in->ld_B >= bc && in->ld_C >= bc &&
                     (in->gate == nullptr || in->ld_gate >= c),
                 "%s: a row pitch is smaller than its row", who);
+    SRX_REQUIRE(pitch_fits(in->ld_x, s->n_channels, dtype, 4) && pitch_fits(in->ld_dt, s->n_channels, dtype, 4) && pitch_fits(in->ld_B, bc, dtype, 16) &&
+                    pitch_fits(in->ld_C, bc, dtype, 16) && (in->gate == nullptr || pitch_fits(in->ld_gate, s->n_channels, dtype, 4)),
+                "%s: a row pitch of about 2^30 bytes (B, C: 2^28) or more", who);
     return SRX_OK;
 }
 
@@ -47,21 +57,18 @@ ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, i
     p.frames = frames;
     const int64_t simds = (int64_t)h->n_cu * 4;
     auto blocks_of = [&](int wide) { return (int64_t)s->n_groups * ((p.per_group + 16 * wide - 1) / (16 * wide)); };
-    // Channels of a lane: as many as leave every SIMD several waves (a frame's work beside the exponentials is
-    // smaller for wide lanes); the registers of 32 and 64 states leave room for fewer.
-    const int most = s->n_states <= 16 ? 4 : s->n_states <= 32 ? 2 : 1;
-    const int least = s->n_states <= 8 ? 4 : 1;
-    p.wide = most;
-    if (train && s->n_states > 8 && s->n_states <= 16) p.wide = 2;
-    while (p.wide > least && utts * blocks_of(p.wide) < 4 * simds) p.wide /= 2;
+    // Two channels a lane, or one where two leave too few waves (the work beside the exponentials is smaller for
+    // two) and from 17 states on, whose registers leave no room for more.
+    p.wide = s->n_states <= 4 ? 4 : 2;
+    if (s->n_states > 16 || (s->n_states > 8 && utts * blocks_of(2) < 2 * simds)) p.wide = 1;
     p.group_blocks = (p.per_group + 16 * p.wide - 1) / (16 * p.wide);
     p.blocks = p.group_blocks * s->n_groups;
     // Whole utterances where they alone give every SIMD a wave; else pieces, whose states are computed twice.
     p.segment = 0;
     p.units = utts;
-    if (utts > 0 && utts * p.blocks < simds) {
+    if (utts > 0 && utts * p.blocks < (getenv("TSP") ? atoi(getenv("TSP")) : simds)) {
         const int64_t even = frames * p.blocks / (4 * simds);
-        const int64_t segment = round_up(even > 64 ? even : 64, 16);
+        const int64_t segment = getenv("TSEG") ? atoi(getenv("TSEG")) : round_up(even > 64 ? even : 64, 16);
         if (frames / utts > 2 * segment) {
             p.segment = segment;
             p.units = frames / segment + utts;
@@ -169,7 +176,8 @@ int srx_selective_scan(srx_handle_t h, const srx_scan_t* s, const srx_scan_input
     if (n_utts == 0) return SRX_OK;
     SRX_REQUIRE(utt_offsets != nullptr, "%s: NULL utterance offsets", who);
     SRX_REQUIRE(n_frames == 0 || y != nullptr, "%s: NULL y", who);
-    SRX_REQUIRE(n_frames == 0 || ld_y >= s->n_channels, "%s: a row pitch is smaller than its row", who);
+    SRX_REQUIRE(n_frames == 0 || (ld_y >= s->n_channels && pitch_fits(ld_y, s->n_channels, dtype, 4)),
+                "%s: a row pitch is smaller than its row, or 2^30 bytes or more", who);
     ScanParams p = params_for(h, s, n_utts, n_frames, saved != nullptr);
     const int64_t need = carve(p, false, workspace);
     SRX_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need),
@@ -230,6 +238,9 @@ int srx_selective_scan_backward(srx_handle_t h, const srx_scan_t* s, const srx_s
         SRX_REQUIRE(ld_dy >= c && grads->ld_dx >= c && grads->ld_ddt >= c && grads->ld_dB >= bc &&
                         grads->ld_dC >= bc && (in->gate == nullptr || grads->ld_dgate >= c),
                     "%s: a row pitch is smaller than its row", who);
+        SRX_REQUIRE(pitch_fits(ld_dy, s->n_channels, dtype, 4) && pitch_fits(grads->ld_dx, s->n_channels, dtype, 4) &&
+                        pitch_fits(grads->ld_ddt, s->n_channels, dtype, 4) && (in->gate == nullptr || pitch_fits(grads->ld_dgate, s->n_channels, dtype, 4)),
+                    "%s: a row pitch of 2^30 bytes or more", who);
     }
     ScanParams p = params_for(h, s, n_utts, n_frames, true);
     const int64_t need = carve(p, true, workspace);
