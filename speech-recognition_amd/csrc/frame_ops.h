@@ -70,6 +70,19 @@ __device__ __forceinline__ void store_some(T* p, const Pack<T, V>& v, int n) {
         if (i < n) p[i] = v.v[i];
 }
 
+// The same where a condition that holds for the whole wave says that all V exist: a branch that the wave takes as one, so
+// that a row of such loads stays one run of instructions and all of them are in flight together.
+template <int V, typename T>
+__device__ __forceinline__ Pack<T, V> load_where(bool all, const T* p, int n) {
+    if (all) return load_pack<V>(p);
+    return load_some<V>(p, n);
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_where(bool all, T* p, const Pack<T, V>& v, int n) {
+    if (all) store_pack(p, v);
+    else store_some(p, v, n);
+}
+
 // e^x by the hardware's 2^x; the part of x log2(e) that its rounding to 32 bits drops is put
 // back to first order, so that the relative error does not grow with |x|.
 __device__ __forceinline__ float exp_f32(float x) {
@@ -155,6 +168,32 @@ __device__ __forceinline__ float wave_sum(float v) {
     v = row16_sum(v);
     v = rows_sum(v, v);
     return halves_sum(v, v);
+}
+
+// Parts [parts][columns] added up in a fixed order, 32 columns a workgroup and every 32nd part a thread; `store` takes
+// a column's sum.
+constexpr int kSumThreads = 1024;
+template <typename F>
+__device__ __forceinline__ void sum_parts(const float* part, int64_t parts, int64_t columns, F store) {
+    __shared__ double sums[32][33];
+    const int at = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int64_t column = (int64_t)blockIdx.x * 32 + at;
+    double s = 0.0;
+    if (column < columns) {
+        int64_t k = slice;
+        for (; k + 96 < parts; k += 128) {               // four loads in flight
+            const float a = part[k * columns + column], b = part[(k + 32) * columns + column];
+            const float c = part[(k + 64) * columns + column], d = part[(k + 96) * columns + column];
+            s += ((double)a + (double)b) + ((double)c + (double)d);
+        }
+        for (; k < parts; k += 32) s += (double)part[k * columns + column];
+    }
+    sums[slice][at] = s;
+    __syncthreads();
+    if (slice != 0 || column >= columns) return;
+    s = 0.0;
+    for (int k = 0; k < 32; ++k) s += sums[k][at];
+    store(column, s);
 }
 
 // Entry points run on the context's device and leave the caller's current device alone.

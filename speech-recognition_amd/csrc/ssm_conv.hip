@@ -10,7 +10,7 @@ using namespace srx_frames;
 namespace {
 
 constexpr int kConvMaxWidth = 8;
-constexpr int kConvPiece = 16;          // frames that a thread walks over
+constexpr int kConvPiece = 32;          // frames that a thread walks over
 
 struct ConvParams {
     const float *weight, *bias;
@@ -92,17 +92,27 @@ __device__ __forceinline__ Pack<T, V> conv_row(const ConvParams& p, const ConvPi
     return load_some<V>((const T*)p.state_in + (w.utt * (W - 1) + place + W - 1) * p.channels + c, left);
 }
 
+// blockDim = (lanes, 256 / lanes), lanes across the channels; neighbouring workgroups have neighbouring channels, so that what
+// runs at the same time covers whole rows and with them all memory channels.  A thread keeps its channels' taps over all the pieces
+// that it takes.  The next four frames are on their way while four are computed.
 template <typename T, int V, int W>
-__global__ __launch_bounds__(256) void conv_forward_kernel(ConvParams p, int64_t pieces, int vectors) {
-    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < pieces * vectors; id += (int64_t)gridDim.x * 256) {
-        const int64_t number = id / vectors;
-        const int c = (int)(id - number * vectors) * V;
+__global__ __launch_bounds__(256) void conv_forward_kernel(ConvParams p, int64_t pieces) {
+    const int c = (int)(blockIdx.x * blockDim.x + threadIdx.x) * V, left = p.channels - c;
+    if (left <= 0) return;
+    const bool all = (int)((blockIdx.x + 1) * blockDim.x) * V <= p.channels;      // (for the whole workgroup)
+    ConvTaps<T, V, W> taps;
+    taps.load(p, c, left);
+    for (int64_t number = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; number < pieces;
+         number += (int64_t)gridDim.y * blockDim.y) {
         ConvPiece w;
         if (!conv_piece(p, number, w)) continue;
-        const int left = p.channels - c;
-        ConvTaps<T, V, W> taps;
-        taps.load(p, c, left);
         Pack<T, V> row[W];                       // the frames under the filter, oldest first
+        constexpr int AHEAD = 4;
+        Pack<T, V> in[AHEAD], next[AHEAD];
+        const T* x = (const T*)p.x + c;
+        if (w.first < w.last)
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) next[i] = load_where<V>(all, x + min(w.first + i, w.last - 1) * p.ld_x, left);
         const int64_t place = w.first - w.begin;
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) row[k + 1] = conv_row<T, V, W>(p, w, place - (W - 1) + k, c, left);
@@ -122,12 +132,13 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvParams p, int64_t
                 store_some((T*)p.state_out + (w.utt * (W - 1) + j) * p.channels + c, v, left);
             }
         }
-        constexpr int AHEAD = 4;                  // loads in flight
         for (int64_t t0 = w.first; t0 < w.last; t0 += AHEAD) {
-            Pack<T, V> in[AHEAD];
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-                in[i] = load_some<V>((const T*)p.x + min(t0 + i, w.last - 1) * p.ld_x + c, left);
+            for (int i = 0; i < AHEAD; ++i) in[i] = next[i];
+            if (t0 + AHEAD < w.last)
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i)
+                    next[i] = load_where<V>(all, x + min(t0 + AHEAD + i, w.last - 1) * p.ld_x, left);
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
 #pragma unroll
@@ -138,7 +149,7 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvParams p, int64_t
                 Pack<T, V> out;
 #pragma unroll
                 for (int v = 0; v < V; ++v) out.v[v] = (T)(p.act == SRX_SILU ? s[v] * sigmoid_f32(s[v]) : s[v]);
-                if (t0 + i < w.last) store_some((T*)p.y + (t0 + i) * p.ld_y + c, out, left);
+                if (t0 + i < w.last) store_where(all, (T*)p.y + (t0 + i) * p.ld_y + c, out, left);
             }
         }
     }
@@ -174,7 +185,8 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvParams p, int64_t ro
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void conv_backward_kernel(ConvParams p, int64_t pieces) {
     __shared__ float sums[256 * (W + 1) * V];
-    const int c = (int)(blockIdx.y * blockDim.x + threadIdx.x) * V, left = p.channels - c;
+    const int c = (int)(blockIdx.x * blockDim.x + threadIdx.x) * V, left = p.channels - c;
+    const bool all = (int)((blockIdx.x + 1) * blockDim.x) * V <= p.channels;      // (for the whole workgroup)
     ConvTaps<T, V, W> taps;
     taps.load(p, c, left);
     float dw[W][V], db[V];
@@ -184,8 +196,8 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvParams p, int64_
 #pragma unroll
         for (int k = 0; k < W; ++k) dw[k][v] = 0.0f;
     }
-    for (int64_t number = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; number < pieces;
-         number += (int64_t)gridDim.x * blockDim.y) {
+    for (int64_t number = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; number < pieces;
+         number += (int64_t)gridDim.y * blockDim.y) {
         ConvPiece w;
         if (left <= 0 || !conv_piece(p, number, w)) continue;
         const int64_t place = w.first - w.begin, length = w.end - w.begin;
@@ -205,8 +217,8 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvParams p, int64_
             for (int i = 0; i < AHEAD; ++i) {
                 const int64_t t = min(t0 + i, w.end - 1);
                 if (w.end > w.begin) {
-                    in[i] = load_some<V>((const T*)p.x + t * p.ld_x + c, left);
-                    dy[i] = load_some<V>((const T*)p.dy + t * p.ld_dy + c, left);
+                    in[i] = load_where<V>(all, (const T*)p.x + t * p.ld_x + c, left);
+                    dy[i] = load_where<V>(all, (const T*)p.dy + t * p.ld_dy + c, left);
                 }
             }
 #pragma unroll
@@ -261,7 +273,7 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvParams p, int64_
                 }
 #pragma unroll
                 for (int v = 0; v < V; ++v) out.v[v] = (T)d[v];
-                if (own) store_some((T*)p.dx + (t - (W - 1)) * p.ld_dx + c, out, left);
+                if (own) store_where(all, (T*)p.dx + (t - (W - 1)) * p.ld_dx + c, out, left);
                 else store_some((T*)p.dstate_in + (w.utt * (W - 1) + at + W - 1) * p.channels + c, out, left);
             }
         }
@@ -277,28 +289,19 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvParams p, int64_
     __syncthreads();
     const int wide = lanes * V;
     for (int e = threadIdx.y * lanes + threadIdx.x; e < (W + 1) * wide; e += 256) {
-        const int k = e / wide, at = e - k * wide, channel = (int)blockIdx.y * wide + at;
+        const int k = e / wide, at = e - k * wide, channel = (int)blockIdx.x * wide + at;
         float s = 0.0f;
         for (int y = 0; y < (int)blockDim.y; ++y) s += sums[(y * (W + 1) + k) * wide + at];
-        if (channel < p.channels) p.part[((int64_t)blockIdx.x * (W + 1) + k) * p.channels + channel] = s;
+        if (channel < p.channels) p.part[((int64_t)blockIdx.y * (W + 1) + k) * p.channels + channel] = s;
     }
 }
 
-// Parts added up in a fixed order: 64 columns per workgroup, four rows of parts at a time.
-__global__ __launch_bounds__(256) void conv_sum_kernel(ConvParams p, int width) {
-    __shared__ double sums[4][64];
-    const int columns = (width + 1) * p.channels;
-    const int column = (int)blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
-    double s = 0.0;
-    if (column < columns)
-        for (int64_t part = slice; part < p.parts; part += 4) s += (double)p.part[part * columns + column];
-    sums[slice][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (slice != 0 || column >= columns) return;
-    s = (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
-    const int k = column / p.channels, c = column - k * p.channels;
-    if (k < width) p.dweight[(int64_t)c * width + k] = (float)s;
-    else if (p.dbias != nullptr) p.dbias[c] = (float)s;
+__global__ __launch_bounds__(kSumThreads) void conv_sum_kernel(ConvParams p, int width) {
+    sum_parts(p.part, p.parts, (int64_t)(width + 1) * p.channels, [&](int64_t column, double s) {
+        const int k = (int)(column / p.channels), c = (int)(column - (int64_t)k * p.channels);
+        if (k < width) p.dweight[(int64_t)c * width + k] = (float)s;
+        else if (p.dbias != nullptr) p.dbias[c] = (float)s;
+    });
 }
 
 constexpr int64_t kMostWorkgroups = 1 << 22;
@@ -310,9 +313,10 @@ unsigned conv_grid(int64_t threads) {
 int64_t conv_pieces(int64_t utts, int64_t frames) { return utts == 0 ? 0 : frames / kConvPiece + utts; }
 
 constexpr int kBackwardVector = 4;
+constexpr int kForwardVector = 4;
 
-int conv_lanes(int channels) {
-    const int vectors = (channels + kBackwardVector - 1) / kBackwardVector;
+int conv_lanes(int channels, int v) {
+    const int vectors = (channels + v - 1) / v;
     int lanes = 8;
     while (lanes < 64 && lanes < vectors) lanes *= 2;
     return lanes;
@@ -320,13 +324,13 @@ int conv_lanes(int channels) {
 // Workgroups along the pieces: enough to fill the chip several times over, and few enough frames per thread
 // (512 at most) that the 32-bit sums of the taps' gradients stay exact to a few units of rounding.
 int64_t conv_parts(const srx_context* h, int channels, int64_t utts, int64_t frames) {
-    const int lanes = conv_lanes(channels), rows = 256 / lanes;
+    const int lanes = conv_lanes(channels, kBackwardVector), rows = 256 / lanes;
     const int64_t across = (channels + lanes * kBackwardVector - 1) / (lanes * kBackwardVector);
     const int64_t groups = (conv_pieces(utts, frames) + rows - 1) / rows;
     const int64_t fill = ((int64_t)h->n_cu * 8 + across - 1) / across;
     const int64_t exact = (groups + 31) / 32;
     const int64_t parts = groups < fill ? groups : fill > exact ? fill : exact;
-    return parts < 1 ? 1 : parts;
+    return parts < 1 ? 1 : parts < 65535 ? parts : 65535;              // (a grid's second dimension)
 }
 
 enum ConvWhat { FORWARD, STEP, BACKWARD };
@@ -339,13 +343,17 @@ int conv_launch(const ConvParams& p, ConvWhat what, hipStream_t st) {
     if (what == STEP) {
         conv_step_kernel<T, V, W><<<conv_grid(p.utts * vectors), 256, 0, st>>>(p, p.utts, vectors);
     } else if (what == FORWARD) {
-        conv_forward_kernel<T, V, W><<<conv_grid(pieces * vectors), 256, 0, st>>>(p, pieces, vectors);
+        constexpr int FV = kForwardVector;
+        const int lanes = conv_lanes(p.channels, FV), rows = 256 / lanes;
+        const int64_t across = (p.channels + lanes * FV - 1) / (lanes * FV), groups = (pieces + rows - 1) / rows;
+        const int64_t fill = (p.parts + across - 1) / across;       // (parts: the workgroups that the chip holds)
+        conv_forward_kernel<T, FV, W><<<dim3((unsigned)across, (unsigned)(groups < fill ? groups : fill)), dim3(lanes, rows), 0, st>>>(p, pieces);
     } else {
-        const int lanes = conv_lanes(p.channels);
+        const int lanes = conv_lanes(p.channels, kBackwardVector);
         const int across = (p.channels + lanes * kBackwardVector - 1) / (lanes * kBackwardVector);
-        conv_backward_kernel<T, kBackwardVector, W><<<dim3((unsigned)p.parts, across), dim3(lanes, 256 / lanes), 0, st>>>(p, pieces);
+        conv_backward_kernel<T, kBackwardVector, W><<<dim3((unsigned)across, (unsigned)p.parts), dim3(lanes, 256 / lanes), 0, st>>>(p, pieces);
         SRX_HIP(hipGetLastError());
-        conv_sum_kernel<<<((W + 1) * p.channels + 63) / 64, 256, 0, st>>>(p, W);
+        conv_sum_kernel<<<((W + 1) * p.channels + 31) / 32, kSumThreads, 0, st>>>(p, W);
     }
     SRX_HIP(hipGetLastError());
     return SRX_OK;
@@ -422,6 +430,7 @@ int srx_causal_conv(srx_handle_t h, const srx_conv_t* conv, int dtype, const voi
     p.state_out = state_out;
     p.y = y;
     p.ld_y = ld_y;
+    p.parts = (int64_t)h->n_cu * 16;
     DeviceGuard guard(h->device);
     if (guard.rc) return guard.rc;
     return conv_run(p, conv->width, dtype, FORWARD, (hipStream_t)stream);

@@ -48,41 +48,46 @@ def _on_device(ctx, t, name):
                          "under torch.no_grad(), and use the *_backward functions")
 
 
-def _rows(ctx, t, name, shape, dtype):
-    """Checks a matrix of rows, (n, ...) with contiguous rows; returns its pitch in elements."""
+# (The checks come before every launch, and a launch for a few live streams takes microseconds: what is in order is
+# passed with one test of each property, the words for what is not are found afterwards.)
+
+def _rows(ctx, t, name, shape, dtype, width):
+    """Checks a matrix of rows, (n, ...) with `width` contiguous values a row; returns its pitch in elements."""
     _on_device(ctx, t, name)
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"Shape mismatch: {name} is {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    width = 1
-    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        if size > 1 and stride != width:
-            raise ValueError(f"the rows of {name} must be contiguous")
-        width *= size
-    if t.shape[0] <= 1:
+    if t.is_contiguous():
         return width
-    if t.stride(0) < width:
+    strides, want = t.stride(), 1
+    for size, stride in zip(shape[:0:-1], strides[:0:-1]):
+        if size > 1 and stride != want:
+            raise ValueError(f"the rows of {name} must be contiguous")
+        want *= size
+    if shape[0] <= 1:
+        return width
+    if strides[0] < width:
         raise ValueError(f"the rows of {name} overlap")
-    return t.stride(0)
+    return strides[0]
 
 
 def _parameter(ctx, t, name, shape):
     if t is None:
         return None
     _on_device(ctx, t, name)
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"Shape mismatch: {name} is {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != torch.float32:
         raise ValueError(f"{name} must be float32, got {t.dtype}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _state(ctx, t, name, shape, dtype):
     if t is None:
         return None
     _on_device(ctx, t, name)
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {tuple(shape)} {dtype} tensor")
     return t
 
@@ -106,40 +111,40 @@ def _offsets(ctx, offsets, n_frames):
 
 
 def _extent(t):
-    """(first byte, byte behind the last, bytes between rows, bytes of a row)"""
-    size = t.element_size()
-    width = int(np.prod(t.shape[1:], dtype=np.int64)) * size
-    pitch = t.stride(0) * size if t.dim() > 0 and t.shape[0] > 1 else width
-    return t.data_ptr(), t.data_ptr() + (t.shape[0] - 1) * pitch + width, pitch, width
+    """(first byte, byte behind the last)"""
+    begin, size = t.data_ptr(), t.element_size()
+    if t.is_contiguous():
+        return begin, begin + t.numel() * size
+    return begin, begin + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * size
 
 
 def _apart(out, name, *inputs):
     """Refuses a result that shares memory with an input (rows of one wider matrix, side by side, do not)."""
     if out.numel() == 0:
         return
-    a0, a1, pitch, width = _extent(out)
+    a0, a1 = _extent(out)
     for t in inputs:
-        if t is None or t.numel() == 0:
+        if t is None or t.data_ptr() >= a1 or t.numel() == 0:
             continue
-        b0, b1, other, wide = _extent(t)
-        if b0 >= a1 or a0 >= b1:
+        b0, b1 = _extent(t)
+        if a0 >= b1:
             continue
-        if pitch == other and width < pitch:
-            if width <= (b0 - a0) % pitch <= pitch - wide:
+        if out.dim() > 1 and t.dim() > 1 and out.shape[0] > 1 and t.shape[0] > 1:
+            pitch, other = out.stride(0) * out.element_size(), t.stride(0) * t.element_size()
+            width = a1 - a0 - (out.shape[0] - 1) * pitch
+            wide = b1 - b0 - (t.shape[0] - 1) * other
+            if pitch == other and 0 < width < pitch and width <= (b0 - a0) % pitch <= pitch - wide:
                 continue
         raise ValueError(f"{name} shares memory with an input")
 
 
 def _out(ctx, out, name, shape, dtype, inputs):
+    """(the result's tensor, its pitch in elements)"""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=ctx.device)
-    _rows(ctx, out, name, shape, dtype)
+        return torch.empty(shape, dtype=dtype, device=ctx.device), shape[1]
+    pitch = _rows(ctx, out, name, shape, dtype, shape[1])
     _apart(out, name, *inputs)
-    return out
-
-
-def _pitch(t, width):
-    return t.stride(0) if t.shape[0] > 1 else width
+    return out, pitch
 
 
 def _address(t):
@@ -158,35 +163,34 @@ class _ScanCall:
     """The checked arguments that the three forms of the scan have in common."""
 
     def __init__(self, ctx, x, dt, A, B, C_, skip, gate, dt_bias, dt_softplus):
-        _on_device(ctx, x, "x")
-        if x.dim() != 2:
-            raise ValueError("x must be 2-D (n_frames, n_channels)")
-        self.code = _code(x, "x")
-        n, c = x.shape
-        _on_device(ctx, A, "A")
-        if A.dim() != 2 or A.shape[0] != c:
-            raise ValueError(f"Shape mismatch: A is {tuple(A.shape)}, expected ({c}, n_states)")
-        states = int(A.shape[1])
-        _on_device(ctx, B, "B")
-        if B.dim() not in (2, 3):
-            raise ValueError("B must be (n_frames, n_states) or (n_frames, n_groups, n_states)")
-        groups = int(B.shape[1]) if B.dim() == 3 else 1
+        for t, name, dims, words in ((x, "x", (2,), "(n_frames, n_channels)"), (A, "A", (2,), "(n_channels, n_states)"),
+                                     (B, "B", (2, 3), "(n_frames, n_states) or (n_frames, n_groups, n_states)")):
+            if not isinstance(t, torch.Tensor):
+                raise ValueError(f"{name} must be a tensor on {ctx.device}")
+            if t.dim() not in dims:
+                raise ValueError(f"{name} must be {'2-D ' if dims == (2,) else ''}{words}")
+        self.code, dtype = _code(x, "x"), x.dtype
+        n, c = rows = tuple(x.shape)
+        states = A.shape[1]
+        groups = B.shape[1] if B.dim() == 3 else 1
         if groups < 1 or c % groups:
             raise ValueError(f"Shape mismatch: {c} channels in {groups} groups")
         wide = (n, groups, states) if B.dim() == 3 else (n, states)
-        self.n, self.channels, self.states, self.groups = int(n), int(c), states, groups
-        self.dtype, self.wide = x.dtype, wide
+        self.n, self.channels, self.states, self.groups = n, c, states, groups
+        self.dtype, self.wide = dtype, wide
         A = _parameter(ctx, A, "A", (c, states))
         skip = _parameter(ctx, skip, "skip", (c,))
         dt_bias = _parameter(ctx, dt_bias, "dt_bias", (c,))
         self.keep = (A, skip, dt_bias)                   # (copies, where a parameter was not contiguous)
-        self.scan = _lib.Scan(c, states, groups, int(bool(dt_softplus)), A.data_ptr(), _address(skip),
+        self.scan = _lib.Scan(c, states, groups, 1 if dt_softplus else 0, A.data_ptr(), _address(skip),
                               _address(dt_bias))
         self.inputs = (x, dt, B, C_, gate)
-        lds = (_rows(ctx, x, "x", (n, c), x.dtype), _rows(ctx, dt, "dt", (n, c), x.dtype),
-               _rows(ctx, B, "B", wide, x.dtype), _rows(ctx, C_, "C", wide, x.dtype),
-               0 if gate is None else _rows(ctx, gate, "gate", (n, c), x.dtype))
-        self.rows = _lib.ScanInputs(x.data_ptr(), dt.data_ptr(), B.data_ptr(), C_.data_ptr(), _address(gate), *lds)
+        bc = groups * states
+        self.rows = _lib.ScanInputs(
+            x.data_ptr(), dt.data_ptr(), B.data_ptr(), C_.data_ptr(), _address(gate),
+            _rows(ctx, x, "x", rows, dtype, c), _rows(ctx, dt, "dt", rows, dtype, c),
+            _rows(ctx, B, "B", wide, dtype, bc), _rows(ctx, C_, "C", wide, dtype, bc),
+            0 if gate is None else _rows(ctx, gate, "gate", rows, dtype, c))
 
 
 def selective_scan(ctx, x, dt, A, B, C, offsets=None, skip=None, gate=None, dt_bias=None, dt_softplus=True,
@@ -207,7 +211,7 @@ def selective_scan(ctx, x, dt, A, B, C, offsets=None, skip=None, gate=None, dt_b
     utts = off.numel() - 1
     shape = (utts, a.channels, a.states)
     state = _state(ctx, state, "state", shape, torch.float32)
-    y = _out(ctx, out, "out", (a.n, a.channels), a.dtype, a.inputs)
+    y, ld_y = _out(ctx, out, "out", (a.n, a.channels), a.dtype, a.inputs)
     if state_out is None:
         state_out = torch.empty(shape, dtype=torch.float32, device=ctx.device)
     else:
@@ -219,7 +223,7 @@ def selective_scan(ctx, x, dt, A, B, C, offsets=None, skip=None, gate=None, dt_b
                             device=ctx.device)
     ws = _workspace(ctx, lib.srx_selective_scan_workspace(ctx.handle, _ref(a.scan), utts, a.n))
     check(lib.srx_selective_scan(ctx.handle, _ref(a.scan), _ref(a.rows), a.code, off.data_ptr(), utts, a.n,
-                                 _address(state), state_out.data_ptr(), y.data_ptr(), _pitch(y, a.channels),
+                                 _address(state), state_out.data_ptr(), y.data_ptr(), ld_y,
                                  _address(saved), _address(ws), 0 if ws is None else ws.numel(),
                                  ctx.stream_ptr()), "srx_selective_scan")
     return (y, state_out, saved) if save else (y, state_out)
@@ -237,7 +241,7 @@ def selective_scan_backward(ctx, dy, x, dt, A, B, C, offsets=None, skip=None, ga
     shape = (utts, a.channels, a.states)
     state = _state(ctx, state, "state", shape, torch.float32)
     dstate_out = _state(ctx, dstate_out, "dstate_out", shape, torch.float32)
-    ld_dy = _rows(ctx, dy, "dy", (a.n, a.channels), a.dtype)
+    ld_dy = _rows(ctx, dy, "dy", (a.n, a.channels), a.dtype, a.channels)
     size = lib.srx_selective_scan_saved(_ref(a.scan), utts, a.n)
     if saved is None:
         saved = selective_scan(ctx, x, dt, A, B, C, off, skip, gate, dt_bias, dt_softplus, state, save=True)[2]
@@ -277,9 +281,9 @@ def selective_scan_step(ctx, state, x, dt, A, B, C, skip=None, gate=None, dt_bia
         raise ValueError("state must be given")
     _state(ctx, state, "state", (a.n, a.channels, a.states), torch.float32)
     _apart(state, "state", *a.inputs, *a.keep)
-    y = _out(ctx, out, "out", (a.n, a.channels), a.dtype, (*a.inputs, state))
+    y, ld_y = _out(ctx, out, "out", (a.n, a.channels), a.dtype, (*a.inputs, state))
     check(lib.srx_selective_scan_step(ctx.handle, _ref(a.scan), _ref(a.rows), a.code, a.n, state.data_ptr(),
-                                      y.data_ptr(), _pitch(y, a.channels), ctx.stream_ptr()),
+                                      y.data_ptr(), ld_y, ctx.stream_ptr()),
           "srx_selective_scan_step")
     return y
 
@@ -288,15 +292,13 @@ def selective_scan_step(ctx, state, x, dt, A, B, C, skip=None, gate=None, dt_bia
 
 class _ConvCall:
     def __init__(self, ctx, x, weight, bias, activation):
-        _on_device(ctx, x, "x")
-        if x.dim() != 2:
-            raise ValueError("x must be 2-D (n_frames, n_channels)")
+        if not isinstance(x, torch.Tensor) or x.dim() != 2:
+            raise ValueError("x must be a 2-D (n_frames, n_channels) tensor")
         self.code = _code(x, "x")
-        self.n, self.channels = (int(v) for v in x.shape)
-        _on_device(ctx, weight, "weight")
-        if weight.dim() != 2:
-            raise ValueError("weight must be (n_channels, width)")
-        self.width = int(weight.shape[1])
+        self.n, self.channels = rows = tuple(x.shape)
+        if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+            raise ValueError("weight must be a (n_channels, width) tensor")
+        self.width = weight.shape[1]
         if not 1 <= self.width <= 8:
             raise ValueError(f"width {self.width} outside [1, 8]")
         if activation not in _ACTIVATIONS:
@@ -304,7 +306,7 @@ class _ConvCall:
         weight = _parameter(ctx, weight, "weight", (self.channels, self.width))
         bias = _parameter(ctx, bias, "bias", (self.channels,))
         self.keep = (weight, bias)
-        self.ld = _rows(ctx, x, "x", (self.n, self.channels), x.dtype)
+        self.ld = _rows(ctx, x, "x", rows, x.dtype, self.channels)
         self.conv = _lib.Conv(self.channels, self.width, _ACTIVATIONS[activation], 0, weight.data_ptr(),
                               _address(bias))
 
@@ -319,14 +321,14 @@ def causal_conv(ctx, x, weight, offsets=None, bias=None, activation=None, state=
     utts = off.numel() - 1
     shape = (utts, a.width - 1, a.channels)
     state = _state(ctx, state, "state", shape, x.dtype)
-    y = _out(ctx, out, "out", (a.n, a.channels), x.dtype, (x, *a.keep, state))
+    y, ld_y = _out(ctx, out, "out", (a.n, a.channels), x.dtype, (x, *a.keep, state))
     if state_out is None:
         state_out = torch.empty(shape, dtype=x.dtype, device=ctx.device)
     else:
         _state(ctx, state_out, "state_out", shape, x.dtype)
         _apart(state_out, "state_out", x, *a.keep, y, None if state_out is state else state)
     check(lib.srx_causal_conv(ctx.handle, _ref(a.conv), a.code, x.data_ptr(), a.ld, off.data_ptr(), utts, a.n,
-                              _address(state), state_out.data_ptr(), y.data_ptr(), _pitch(y, a.channels),
+                              _address(state), state_out.data_ptr(), y.data_ptr(), ld_y,
                               ctx.stream_ptr()), "srx_causal_conv")
     return y, state_out
 
@@ -341,7 +343,7 @@ def causal_conv_backward(ctx, dy, x, weight, offsets=None, bias=None, activation
     shape = (utts, a.width - 1, a.channels)
     state = _state(ctx, state, "state", shape, x.dtype)
     dstate_out = _state(ctx, dstate_out, "dstate_out", shape, x.dtype)
-    ld_dy = _rows(ctx, dy, "dy", (a.n, a.channels), x.dtype)
+    ld_dy = _rows(ctx, dy, "dy", (a.n, a.channels), x.dtype, a.channels)
     grads = {"x": torch.empty((a.n, a.channels), dtype=x.dtype, device=ctx.device),
              "weight": torch.empty((a.channels, a.width), dtype=torch.float32, device=ctx.device),
              "bias": None if bias is None else torch.empty((a.channels,), dtype=torch.float32, device=ctx.device),
@@ -363,9 +365,9 @@ def causal_conv_step(ctx, state, x, weight, bias=None, activation=None, out=None
         raise ValueError("state must be given")
     _state(ctx, state, "state", (a.n, a.width - 1, a.channels), x.dtype)
     _apart(state, "state", x, *a.keep)
-    y = _out(ctx, out, "out", (a.n, a.channels), x.dtype, (x, *a.keep, state))
+    y, ld_y = _out(ctx, out, "out", (a.n, a.channels), x.dtype, (x, *a.keep, state))
     check(lib.srx_causal_conv_step(ctx.handle, _ref(a.conv), a.code, x.data_ptr(), a.ld, a.n, state.data_ptr(),
-                                   y.data_ptr(), _pitch(y, a.channels), ctx.stream_ptr()), "srx_causal_conv_step")
+                                   y.data_ptr(), ld_y, ctx.stream_ptr()), "srx_causal_conv_step")
     return y
 
 
@@ -375,29 +377,26 @@ def layer_norm(ctx, x, weight=None, bias=None, eps=1e-5, out=None):
     """y = (x - mean) rstd weight + bias for every row of x (n, features), rstd = 1 / sqrt(variance + eps) with the
     variance over n values.  Returns (y, mean, rstd), the last two (n,) float32: what
     ``layer_norm_backward`` wants of this pass."""
-    _on_device(ctx, x, "x")
-    if x.dim() != 2:
-        raise ValueError("x must be 2-D (n_rows, n_features)")
-    n, d = (int(v) for v in x.shape)
-    code, ld = _code(x, "x"), _rows(ctx, x, "x", (n, d), x.dtype)
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a 2-D (n_rows, n_features) tensor")
+    n, d = rows = tuple(x.shape)
+    code, ld = _code(x, "x"), _rows(ctx, x, "x", rows, x.dtype, d)
     weight, bias = _parameter(ctx, weight, "weight", (d,)), _parameter(ctx, bias, "bias", (d,))
-    y = _out(ctx, out, "out", (n, d), x.dtype, (x, weight, bias))
-    mean = torch.empty((n,), dtype=torch.float32, device=ctx.device)
-    rstd = torch.empty((n,), dtype=torch.float32, device=ctx.device)
+    y, ld_y = _out(ctx, out, "out", rows, x.dtype, (x, weight, bias))
+    mean, rstd = torch.empty((2, n), dtype=torch.float32, device=ctx.device).unbind(0)
     check(lib.srx_layer_norm(ctx.handle, x.data_ptr(), ld, code, n, d, _address(weight), _address(bias), float(eps),
-                             y.data_ptr(), _pitch(y, d), mean.data_ptr(), rstd.data_ptr(), ctx.stream_ptr()),
+                             y.data_ptr(), ld_y, mean.data_ptr(), rstd.data_ptr(), ctx.stream_ptr()),
           "srx_layer_norm")
     return y, mean, rstd
 
 
 def layer_norm_backward(ctx, dy, x, mean, rstd, weight=None):
     """(dx, dweight, dbias) of ``layer_norm`` for the gradient dy of its y; dx in x's type, the others float32."""
-    _on_device(ctx, x, "x")
-    if x.dim() != 2:
-        raise ValueError("x must be 2-D (n_rows, n_features)")
-    n, d = (int(v) for v in x.shape)
-    code, ld = _code(x, "x"), _rows(ctx, x, "x", (n, d), x.dtype)
-    ld_dy = _rows(ctx, dy, "dy", (n, d), x.dtype)
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a 2-D (n_rows, n_features) tensor")
+    n, d = rows = tuple(x.shape)
+    code, ld = _code(x, "x"), _rows(ctx, x, "x", rows, x.dtype, d)
+    ld_dy = _rows(ctx, dy, "dy", rows, x.dtype, d)
     mean, rstd = _parameter(ctx, mean, "mean", (n,)), _parameter(ctx, rstd, "rstd", (n,))
     weight = _parameter(ctx, weight, "weight", (d,))
     dx = torch.empty((n, d), dtype=x.dtype, device=ctx.device)
@@ -415,14 +414,21 @@ def layer_norm_backward(ctx, dy, x, mean, rstd, weight=None):
 
 def _dense(t):
     """Whether a tensor's values fill their memory without gaps, in whatever order."""
-    if t.is_contiguous():
-        return True
+    if t.layout != torch.strided:
+        return False
     want = 1
     for stride, size in sorted((st, sz) for sz, st in zip(t.shape, t.stride()) if sz > 1):
         if stride != want:
             return False
         want *= size
     return True
+
+
+def _codes(tensors, name):
+    try:
+        return [_CODES[t.dtype] for t in tensors]
+    except KeyError:
+        return [_code(t, f"{name}[{i}]") for i, t in enumerate(tensors)]
 
 
 def clip_gradients(ctx, grads, max_norm, out=None):
@@ -437,21 +443,26 @@ def clip_gradients(ctx, grads, max_norm, out=None):
     if outs is not None and len(outs) != len(grads):
         raise ValueError(f"{len(grads)} gradients but {len(outs)} outputs")
     device, n = ctx.device, len(grads)
-    for i, t in enumerate(grads):
-        _on_device(ctx, t, f"grads[{i}]")
-        if t.layout != torch.strided or not _dense(t):
-            raise ValueError(f"grads[{i}] must fill its memory without gaps")
-    counts = (C.c_int64 * max(n, 1))(*[t.numel() for t in grads])
-    tensors = (C.c_void_p * max(n, 1))(*[t.data_ptr() for t in grads])
-    dtypes = (C.c_int32 * max(n, 1))(*[_code(t, "a gradient") for t in grads])
+    for name, tensors in (("grads", grads), ("out", outs or ())):
+        # (in order: passed by one look at each property of all; else the first that is not is found)
+        if not (all([isinstance(t, torch.Tensor) for t in tensors]) and {t.device for t in tensors} <= {device}
+                and not any([t.requires_grad for t in tensors])):
+            for i, t in enumerate(tensors):
+                _on_device(ctx, t, f"{name}[{i}]")
+        if not all([t.is_contiguous() for t in tensors]):
+            for i, t in enumerate(tensors):
+                if not t.is_contiguous() and not _dense(t):
+                    raise ValueError(f"{name}[{i}] must fill its memory without gaps")
+    sizes = [t.numel() for t in grads]
+    counts, tensors = (C.c_int64 * n)(*sizes), (C.c_void_p * n)(*[t.data_ptr() for t in grads])
+    dtypes = (C.c_int32 * n)(*_codes(grads, "grads"))
     to = to_types = None
     if outs is not None:
         for i, (t, o) in enumerate(zip(grads, outs)):
-            _on_device(ctx, o, f"out[{i}]")
-            if o.shape != t.shape or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous())):
+            if o.shape != t.shape or not (o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride()):
                 raise ValueError(f"out[{i}] must have its gradient's shape and order")
-        to = (C.c_void_p * max(n, 1))(*[o.data_ptr() for o in outs])
-        to_types = (C.c_int32 * max(n, 1))(*[_code(o, "an output") for o in outs])
+        to = (C.c_void_p * n)(*[o.data_ptr() for o in outs])
+        to_types = (C.c_int32 * n)(*_codes(outs, "out"))
     norm = torch.empty((), dtype=torch.float64, device=device)
     ws = _workspace(ctx, lib.srx_clip_gradients_workspace(ctx.handle, n, counts))
     check(lib.srx_clip_gradients(ctx.handle, n, tensors, counts, dtypes, to, to_types, float(max_norm),
