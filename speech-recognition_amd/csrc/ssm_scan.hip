@@ -42,7 +42,7 @@ int check_inputs(const srx_scan_t* s, const srx_scan_inputs_t* in, int dtype, in
     return SRX_OK;
 }
 
-ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, int64_t frames, bool train) {
+ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, int64_t frames) {
     ScanParams p;
     memset(&p, 0, sizeof(p));
     p.A = s->A;
@@ -66,20 +66,29 @@ ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, i
     // Whole utterances where they alone give every SIMD a wave; else pieces, whose states are computed twice.
     p.segment = 0;
     p.units = utts;
-    if (utts > 0 && utts * p.blocks < (getenv("TSP") ? atoi(getenv("TSP")) : simds)) {
+    if (utts > 0 && utts * p.blocks < simds) {
         const int64_t even = frames * p.blocks / (4 * simds);
-        const int64_t segment = getenv("TSEG") ? atoi(getenv("TSEG")) : round_up(even > 64 ? even : 64, 16);
+        const int64_t segment = round_up(even > 64 ? even : 64, 16);
         if (frames / utts > 2 * segment) {
             p.segment = segment;
             p.units = frames / segment + utts;
         }
     }
-    // backward: a wave sums the parameters' gradients over all its units
+    // By falling length where there are more waves than run at full rate at once (fewer do not wait for one another),
+    // utterances to choose from, but not so many that the last ones do not matter, and long enough to be worth it.
+    p.ordered = p.segment == 0 && utts >= kScanOrderedLeast && utts <= kScanOrdered && frames >= 32 * utts &&
+                utts * p.blocks >= 2 * simds;
+    // backward: a wave sums the parameters' gradients over all its units (every parts-th of them: long and short ones)
     p.parts = p.units;
     const int64_t enough = 8 * simds / p.blocks + 1;
     if (p.segment == 0 && p.parts > enough) p.parts = enough;
     if (p.parts < 1) p.parts = 1;
     return p;
+}
+
+int64_t saved_states(const srx_scan_t* s, int64_t utts, int64_t frames) {
+    const int64_t ch = 64, per = s->n_channels / s->n_groups;      // (room for every way to cut the channels)
+    return (frames / kScanSaveEvery + utts) * ((per + ch - 1) / ch * s->n_groups) * ch * block_states(s->n_states);
 }
 
 // Hands out the workspace; with a NULL base it only counts.
@@ -99,6 +108,8 @@ int64_t carve(ScanParams& p, bool backward, void* workspace) {
     if (p.segment != 0) {
         p.seg_state = c.floats(p.units * p.blocks * ch * ns);
         p.seg_sum = c.floats(p.units * p.blocks * ch);
+    } else if (p.ordered && p.saved == nullptr) {
+        p.order = (int*)c.floats(p.utts);
     }
     if (backward) {
         p.part_A = c.floats(p.parts * p.blocks * ch * ns);
@@ -132,14 +143,8 @@ void take_inputs(ScanParams& p, const srx_scan_inputs_t* in) {
 int64_t workspace_bytes_for(srx_handle_t h, const srx_scan_t* s, int64_t utts, int64_t frames, bool backward,
                             const char* who) {
     if (check_scan(h, s, utts, frames, who)) return -1;
-    if (backward) {
-        ScanParams p = params_for(h, s, utts, frames, true);
-        return carve(p, true, nullptr);
-    }
-    // (a pass that saves its states may cut the channels differently)
-    ScanParams p = params_for(h, s, utts, frames, false), q = params_for(h, s, utts, frames, true);
-    const int64_t a = carve(p, false, nullptr), b = carve(q, false, nullptr);
-    return a > b ? a : b;
+    ScanParams p = params_for(h, s, utts, frames);
+    return carve(p, backward, nullptr);
 }
 
 }  // namespace
@@ -152,8 +157,8 @@ int64_t srx_selective_scan_saved(const srx_scan_t* s, int64_t n_utts, int64_t n_
         srx_set_error("srx_selective_scan_saved: Shape mismatch");
         return -1;
     }
-    const int64_t ch = 64, per = s->n_channels / s->n_groups;      // (room for every way to cut the channels)
-    return (n_frames / kScanSaveEvery + n_utts) * ((per + ch - 1) / ch * s->n_groups) * ch * block_states(s->n_states);
+    const bool order = n_utts >= kScanOrderedLeast && n_utts <= kScanOrdered;      // (room for it behind the states)
+    return saved_states(s, n_utts, n_frames) + (order ? n_utts : 0);
 }
 
 int64_t srx_selective_scan_workspace(srx_handle_t h, const srx_scan_t* s, int64_t n_utts, int64_t n_frames) {
@@ -178,7 +183,9 @@ int srx_selective_scan(srx_handle_t h, const srx_scan_t* s, const srx_scan_input
     SRX_REQUIRE(n_frames == 0 || y != nullptr, "%s: NULL y", who);
     SRX_REQUIRE(n_frames == 0 || (ld_y >= s->n_channels && pitch_fits(ld_y, s->n_channels, dtype, 4)),
                 "%s: a row pitch is smaller than its row, or 2^30 bytes or more", who);
-    ScanParams p = params_for(h, s, n_utts, n_frames, saved != nullptr);
+    ScanParams p = params_for(h, s, n_utts, n_frames);
+    p.saved = saved;
+    if (saved != nullptr && p.ordered) p.order = (int*)(saved + saved_states(s, n_utts, n_frames));
     const int64_t need = carve(p, false, workspace);
     SRX_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need),
                 "%s: workspace of %lld bytes, %lld are needed", who, (long long)workspace_bytes, (long long)need);
@@ -188,7 +195,6 @@ int srx_selective_scan(srx_handle_t h, const srx_scan_t* s, const srx_scan_input
     p.state_out = state_out;
     p.y = y;
     p.ld_y = ld_y;
-    p.saved = saved;
     DeviceGuard guard(h->device);
     if (guard.rc) return guard.rc;
     return run(p, dtype, false, (hipStream_t)stream);
@@ -203,7 +209,7 @@ int srx_selective_scan_step(srx_handle_t h, const srx_scan_t* s, const srx_scan_
     if (n_rows == 0) return SRX_OK;
     SRX_REQUIRE(state != nullptr && y != nullptr, "%s: NULL state or y", who);
     SRX_REQUIRE(ld_y >= s->n_channels, "%s: a row pitch is smaller than its row", who);
-    ScanParams p = params_for(h, s, n_rows, n_rows, false);
+    ScanParams p = params_for(h, s, n_rows, n_rows);
     take_inputs(p, in);
     p.y = y;
     p.ld_y = ld_y;
@@ -242,13 +248,14 @@ int srx_selective_scan_backward(srx_handle_t h, const srx_scan_t* s, const srx_s
                         pitch_fits(grads->ld_ddt, s->n_channels, dtype, 4) && (in->gate == nullptr || pitch_fits(grads->ld_dgate, s->n_channels, dtype, 4)),
                     "%s: a row pitch of 2^30 bytes or more", who);
     }
-    ScanParams p = params_for(h, s, n_utts, n_frames, true);
+    ScanParams p = params_for(h, s, n_utts, n_frames);
+    p.saved = const_cast<float*>(saved);     // (the backward kernels only read it)
+    if (p.ordered) p.order = (int*)(p.saved + saved_states(s, n_utts, n_frames));
     const int64_t need = carve(p, true, workspace);
     SRX_REQUIRE(workspace != nullptr && workspace_bytes >= need,
                 "%s: workspace of %lld bytes, %lld are needed", who, (long long)workspace_bytes, (long long)need);
     take_inputs(p, in);
     p.off = utt_offsets;
-    p.saved = const_cast<float*>(saved);     // (the backward kernels only read it)
     p.dy = dy;
     p.ld_dy = ld_dy;
     p.dx = grads->dx;

@@ -171,6 +171,50 @@ def test_scan_long_utterances_in_pieces(sra, ctx, lengths, dtype):
     _check_scan(sra, ctx, off, t, v, dtype, rng)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("c,s,g,gate", [(1650, 16, 3, True), (1665, 16, 1, False), (1700, 7, 2, True)])
+def test_scan_batches_that_fill_the_device(sra, ctx, c, s, g, gate, dtype):
+    """Enough rows for two channels a lane and for utterances taken by their lengths; the longest is not the first, one
+    has no frame, and some are equally long."""
+    rng = np.random.default_rng(c)
+    lengths = rng.integers(5, 80, 40)
+    lengths[[3, 30]], lengths[7], lengths[38] = 20, 0, 90
+    assert lengths.sum() >= 32 * 40
+    off, t, v = _scan_case(rng, lengths, c, s, g, dtype, gate=gate)
+    got = _check_scan(sra, ctx, off, t, v, dtype, rng)
+    y, last = _run_scan(sra, ctx, off, t)           # (without saved states: the order is kept elsewhere)
+    torch = _torch()
+    assert torch.equal(y, got[0]) and torch.equal(last, got[1])
+
+
+def test_scan_more_short_utterances_than_a_wave_takes(sra, ctx):
+    """One wave sums the parameters' gradients over several utterances."""
+    rng = np.random.default_rng(25)
+    off, t, v = _scan_case(rng, rng.integers(0, 5, 300), 2040, 16, 1, "float32")
+    _check_scan(sra, ctx, off, t, v, "float32", rng)
+
+
+@pytest.mark.parametrize("u", [0, 3])
+def test_scan_of_no_frames(sra, ctx, u):
+    """No utterance, or only empty ones: states pass, the parameters' gradients are 0."""
+    torch = _torch()
+    rng = np.random.default_rng(26)
+    off, t, v = _scan_case(rng, [0] * u, 20, 16, 1, "float32")
+    dso = torch.from_numpy(rng.standard_normal((u, 20, 16)).astype(np.float32)).cuda()
+    y, last, g = _run_scan(sra, ctx, off, t, torch.empty(0, 20, device="cuda"), dso)
+    assert y.shape == (0, 20) and torch.equal(last, t["state"])
+    assert torch.equal(g["state"], dso)
+    for k in ("A", "skip", "dt_bias"):
+        assert not g[k].any(), k
+    conv = torch.from_numpy(rng.standard_normal((20, 4)).astype(np.float32)).cuda()
+    o = torch.from_numpy(off).cuda()
+    first = torch.from_numpy(rng.standard_normal((u, 3, 20)).astype(np.float32)).cuda()
+    y, last = sra.causal_conv(ctx, t["x"], conv, o, None, "silu", state=first)
+    assert y.shape == (0, 20) and torch.equal(last, first)
+    g = sra.causal_conv_backward(ctx, y, t["x"], conv, o, None, "silu", state=first)
+    assert not g["weight"].any()
+
+
 @pytest.mark.parametrize("pitch", [2, 3, 5])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_scan_takes_rows_at_any_pitch_and_leaves_others_alone(sra, ctx, dtype, pitch):
