@@ -100,10 +100,17 @@ __device__ __forceinline__ float sigmoid_f32(float x) {
 // of that sum dropped, which for a small e is most of its relative accuracy (steps of 0.001 and less
 // are ordinary); its derivative 1 / u is taken as 1, as the dropped part is below 2^-24.  The exponential is
 // off by |x| 2^-24 of itself, as much as x is when it is itself a rounded sum.  A NaN comes through the exponential.
-__device__ __forceinline__ float softplus_f32(float x) {
+// slope: its derivative, the sigmoid, from the same exponential.
+__device__ __forceinline__ float softplus_f32(float x, float& slope) {
     const float e = __builtin_amdgcn_exp2f(-1.44269504088896341f * fabsf(x));
     const float u = 1.0f + e;
+    const float inverse = __builtin_amdgcn_rcpf(u);
+    slope = x >= 0.0f ? inverse : e * inverse;
     return fmaxf(x, 0.0f) + fmaf(__builtin_amdgcn_logf(u), 0.693147180559945309f, e - (u - 1.0f));
+}
+__device__ __forceinline__ float softplus_f32(float x) {
+    float slope;
+    return softplus_f32(x, slope);
 }
 
 // Makes the wave wait here for the loads into v, and not later, behind stores that follow: loads and stores

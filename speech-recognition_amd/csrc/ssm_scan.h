@@ -44,6 +44,7 @@ struct ScanParams {
     // units: utterances (segment == 0) or pieces of `segment` frames of them
     int64_t units, segment;
     bool ordered;
+    int round;               // utterances that give every CU a workgroup
     int* order;              // [utts] utterances by falling length, or NULL: as they come (the backward pass
                              // takes the forward pass's, behind the saved states)
     // forward
@@ -82,7 +83,11 @@ __device__ __forceinline__ void scan_bounds(const ScanParams& p, int64_t utt, in
 __device__ __forceinline__ bool scan_unit(const ScanParams& p, int64_t unit, ScanUnit& w) {
     int64_t begin, end;
     if (p.segment == 0) {
-        const int64_t utt = p.order != nullptr ? p.order[unit] : unit;
+        int64_t utt = unit;
+        if (p.order != nullptr) {                         // odd rounds the other way round: a long one beside a short one
+            const int round = (int)unit / p.round, end = min((round + 1) * p.round, (int)p.utts);
+            utt = p.order[round & 1 ? end - 1 - ((int)unit - round * p.round) : unit];
+        }
         if (utt < 0 || utt >= p.utts) return false;       // (the saved states were not the forward pass's)
         scan_bounds(p, utt, begin, end);
         w = {utt, begin, begin, end, true, true};
@@ -141,8 +146,10 @@ struct ScanRows {
 };
 
 // The utterances by falling length (the same lengths in their own order): the waves of long ones start first, and the
-// chip is not left waiting for one that began last.  96 utterances of 100 to 300 frames x 1024 channels, 16 states: 117 us
-// as they come, 107 so; utterances of equal length pay 6 us for this launch.  Every thread
+// chip is not left waiting for one that began last; and as the first rounds of workgroups stay on their CUs side by
+// side, every other round is taken backwards (scan_unit), so that the lengths of a CU's workgroups add up to much the
+// same.  96 utterances of 100 to 300 frames x 1024 channels, 16 states: 117 us as they come, 107 by falling length, 96
+// with the rounds; utterances of equal length pay 6 us for this launch.  Every thread
 // counts the utterances before its own, in one workgroup.
 constexpr int kScanOrderedLeast = 16, kScanOrdered = 1024;
 static __global__ __launch_bounds__(kScanOrdered) void scan_order_kernel(ScanParams p) {
@@ -416,16 +423,22 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
         for (int64_t done = 0; done < frames; done += TILE) {
             const int here = (int)min(frames - done, (int64_t)TILE);       // frames of this tile
             if (done + TILE < frames) reader.next(p, w, frames - done - TILE, next);
+            Pack<float, R> step[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < R; ++r) step[i].v[r] = (float)now.dt[i].v[r] + bias[r];
+            if (p.softplus)                              // (one branch, so that their latencies overlap)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) step[i].v[r] = softplus_f32(step[i].v[r]);
             wave_lds_fence();                            // the last tile has been read
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                Pack<float, R> d, du;
+                Pack<float, R> d = step[i], du;
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const float raw = (float)now.dt[i].v[r] + bias[r];
-                    d.v[r] = p.softplus ? softplus_f32(raw) : raw;
-                    du.v[r] = d.v[r] * (float)now.x[i].v[r];
-                }
+                for (int r = 0; r < R; ++r) du.v[r] = d.v[r] * (float)now.x[i].v[r];
                 if (here < TILE) {                       // a frame behind the last one changes nothing
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
@@ -611,26 +624,6 @@ template <typename T, int R, int S, bool GATE>
 struct ScanOctetRaw {
     Pack<T, R> x[2], dt[2], z[2], dy[2];
     Pack<T, S> b, c;             // (lanes 32 .. 63 the same as lanes 0 .. 31)
-    // x, dt, z and dy are needed at both ends of an octet's work; in between they lie in LDS.
-    static constexpr int kStash = (int)sizeof(Pack<T, R>) < 4 ? 4 : (int)sizeof(Pack<T, R>);       // bytes a lane
-    __device__ __forceinline__ void put(char* at) const {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            __builtin_memcpy(at + (0 + i) * 64 * kStash, &x[i].v, sizeof(x[i].v));
-            __builtin_memcpy(at + (2 + i) * 64 * kStash, &dt[i].v, sizeof(x[i].v));
-            __builtin_memcpy(at + (4 + i) * 64 * kStash, &dy[i].v, sizeof(x[i].v));
-            if (GATE) __builtin_memcpy(at + (6 + i) * 64 * kStash, &z[i].v, sizeof(x[i].v));
-        }
-    }
-    __device__ __forceinline__ void get(const char* at) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            __builtin_memcpy(&x[i].v, at + (0 + i) * 64 * kStash, sizeof(x[i].v));
-            __builtin_memcpy(&dt[i].v, at + (2 + i) * 64 * kStash, sizeof(x[i].v));
-            __builtin_memcpy(&dy[i].v, at + (4 + i) * 64 * kStash, sizeof(x[i].v));
-            if (GATE) __builtin_memcpy(&z[i].v, at + (6 + i) * 64 * kStash, sizeof(x[i].v));
-        }
-    }
     __device__ __forceinline__ void arrived() {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -718,8 +711,8 @@ template <typename T, int R, int S, bool GATE, int MODE, int SUB>
 __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanParams p) {
     constexpr int CH = 16 * R, NS = 4 * S, TILE = kScanSaveEvery;
     constexpr float kLn2 = 0.693147180559945309f;
-    constexpr int kStash = ScanOctetRaw<T, R, S, GATE>::kStash;
-    __shared__ __align__(16) float lds[kScanWaves][TILE * (6 * CH + 4 * NS) + (MODE == 0 ? 64 * (R * S + 2 * R + 2 * kStash) : 0)];
+    constexpr int kKept = GATE ? 6 : 4;  // 2 (x, slope of the step, gradient by the gate over the ungated output)
+    __shared__ __align__(16) float lds[kScanWaves][TILE * (6 * CH + 4 * NS) + (MODE == 0 ? 64 * (R * S + 2 * R + kKept * R) : 0)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* sD = lds[wave];               // steps
     float* sU = sD + TILE * CH;          // step times x
@@ -731,7 +724,8 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
     float* sC = sB + TILE * NS;
     float* oBC = sC + TILE * NS;         // [frame][B, C][state]: sums over the channels
     float* acc = oBC + 2 * TILE * NS;    // [R S + 2 R][64]: dA, dskip, dbias of the frames so far
-    char* stash = (char*)(acc + 64 * (R * S + 2 * R)) + (threadIdx.x & 63) * kStash;
+    // what both ends of an octet's work need of a lane's own frames lies in LDS in between
+    float* kept = acc + 64 * (R * S + 2 * R) + (threadIdx.x & 63) * R;
     const int across = (p.blocks + kScanWaves - 1) / kScanWaves;
     for (int64_t task = blockIdx.x; task < p.parts * across; task += gridDim.x) {
         const int64_t part = task / across;
@@ -807,20 +801,42 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                 const int64_t t0 = u.first + o * TILE;
                 float h0next[R][S];
                 if (MODE == 1 && o > 0) reader.next(p, w, TILE, next);
+                Pack<float, R> step[2], slope[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        step[i].v[r] = (float)now.dt[i].v[r] + bias[r];
+                        slope[i].v[r] = 1.0f;
+                    }
+                if (p.softplus)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            float by;
+                            step[i].v[r] = softplus_f32(step[i].v[r], by);
+                            slope[i].v[r] = by;
+                        }
                 wave_lds_fence();
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    Pack<float, R> d, du, q;
+                    Pack<float, R> d = step[i], du, q, x, by_gate;
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        const float raw = (float)now.dt[i].v[r] + bias[r];
-                        d.v[r] = p.softplus ? softplus_f32(raw) : raw;
-                        du.v[r] = d.v[r] * (float)now.x[i].v[r];
+                        x.v[r] = (float)now.x[i].v[r];
+                        du.v[r] = d.v[r] * x.v[r];
                         q.v[r] = (float)now.dy[i].v[r];
                         if (GATE) {
-                            const float z = (float)now.z[i].v[r];
-                            q.v[r] *= z * sigmoid_f32(z);
+                            const float z = (float)now.z[i].v[r], sig = sigmoid_f32(z), by = q.v[r] * sig;
+                            q.v[r] = by * z;
+                            by_gate.v[r] = fmaf(q.v[r], 1.0f - sig, by);
                         }
+                    }
+                    if (MODE == 0) {
+                        store_pack(kept + i * 64 * R, x);
+                        store_pack(kept + (2 + i) * 64 * R, slope[i]);
+                        if (GATE) store_pack(kept + (4 + i) * 64 * R, by_gate);
                     }
                     if (frames < TILE || !w.full) {      // what does not exist adds nothing to anything
 #pragma unroll
@@ -849,7 +865,6 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                     store_pack(sC + (w.lane & 31) * S, c);
                 }
                 wave_lds_fence();
-                if (MODE == 0) now.put(stash);
                 if (MODE == 1) {
 #pragma unroll
                     for (int j = TILE - 1; j >= 0; --j) {
@@ -954,7 +969,6 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                     }
                 }
                 wave_lds_fence();
-                now.get(stash);
                 const Pack<float, S> sums = load_pack<S>(oBC + w.lane * S);
                 Pack<T, R> vx[2], vt[2], vz[2];
 #pragma unroll
@@ -964,23 +978,21 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                     const Pack<float, R> vd = load_pack<R>(oD + (4 * i + w.row) * CH + w.col * R);
                     Pack<float, R> vy;
                     if (GATE) vy = load_pack<R>(oY + (4 * i + w.row) * CH + w.col * R);
-                    const Pack<float, R> step = load_pack<R>(sD + (4 * i + w.row) * CH + w.col * R);
+                    const Pack<float, R> d = load_pack<R>(sD + (4 * i + w.row) * CH + w.col * R);
                     const Pack<float, R> dp = load_pack<R>(sP + (4 * i + w.row) * CH + w.col * R);
+                    const Pack<float, R> own = load_pack<R>(kept + i * 64 * R), by_step = load_pack<R>(kept + (2 + i) * 64 * R);
+                    Pack<float, R> by_gate;
+                    if (GATE) by_gate = load_pack<R>(kept + (4 + i) * 64 * R);
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        const float x = (float)now.x[i].v[r];
-                        vx[i].v[r] = (T)fmaf(vu.v[r], step.v[r], dp.v[r] * skip[r]);
-                        float v = fmaf(vd.v[r], kLn2, vu.v[r] * x);
-                        if (p.softplus) v *= sigmoid_f32((float)now.dt[i].v[r] + bias[r]);
+                        const float x = own.v[r];
+                        vx[i].v[r] = (T)fmaf(vu.v[r], d.v[r], dp.v[r] * skip[r]);
+                        float v = fmaf(vd.v[r], kLn2, vu.v[r] * x) * by_step.v[r];
                         vt[i].v[r] = (T)v;
                         if (frames < TILE) v = live ? v : 0.0f;
                         dbias[r] += v;
                         dskip[r] = fmaf(dp.v[r], frames < TILE ? (live ? x : 0.0f) : x, dskip[r]);
-                        if (GATE) {
-                            const float z = (float)now.z[i].v[r], sig = sigmoid_f32(z);
-                            const float out = fmaf(skip[r], x, vy.v[r]);
-                            vz[i].v[r] = (T)((float)now.dy[i].v[r] * out * sig * fmaf(z, 1.0f - sig, 1.0f));
-                        }
+                        if (GATE) vz[i].v[r] = (T)(by_gate.v[r] * fmaf(skip[r], x, vy.v[r]));
                     }
                 }
                 held += TILE;

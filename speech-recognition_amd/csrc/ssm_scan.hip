@@ -1,7 +1,6 @@
 // Entry points of the selective state space scan: argument checks, the choice between whole
 // utterances and pieces of them, and the division of the caller's workspace (kernels: ssm_scan.h).
 #include "ssm_scan.h"
-#include <stdlib.h>
 
 namespace {
 
@@ -78,6 +77,8 @@ ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, i
     // utterances to choose from, but not so many that the last ones do not matter, and long enough to be worth it.
     p.ordered = p.segment == 0 && utts >= kScanOrderedLeast && utts <= kScanOrdered && frames >= 32 * utts &&
                 utts * p.blocks >= 2 * simds;
+    const int64_t round = h->n_cu / ((p.blocks + kScanWaves - 1) / kScanWaves);
+    p.round = (int)(round > 1 ? round : 1);
     // backward: a wave sums the parameters' gradients over all its units (every parts-th of them: long and short ones)
     p.parts = p.units;
     const int64_t enough = 8 * simds / p.blocks + 1;
