@@ -20,6 +20,7 @@ Conventions of every function here:
   - gradients are explicit: the ``*_backward`` functions are called with the gradient of the result,
     torch's autograd is not involved (a tensor that requires grad is refused while it records).
 """
+import array
 import ctypes as C
 
 import numpy as np
@@ -38,6 +39,13 @@ def _code(t, name):
         return _CODES[t.dtype]
     except KeyError:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}") from None
+
+
+_TENSORS = {torch.Tensor, torch.nn.Parameter}
+
+
+def _index(ctx):
+    return -1 if ctx.device.index is None else ctx.device.index
 
 
 def _on_device(ctx, t, name):
@@ -139,9 +147,9 @@ def _apart(out, name, *inputs):
 
 
 def _out(ctx, out, name, shape, dtype, inputs):
-    """(the result's tensor, its pitch in elements)"""
+    """(the result's tensor, its pitch in elements); the first input has its type"""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=ctx.device), shape[1]
+        return inputs[0].new_empty(shape), shape[1]
     pitch = _rows(ctx, out, name, shape, dtype, shape[1])
     _apart(out, name, *inputs)
     return out, pitch
@@ -163,14 +171,11 @@ class _ScanCall:
     """The checked arguments that the three forms of the scan have in common."""
 
     def __init__(self, ctx, x, dt, A, B, C_, skip, gate, dt_bias, dt_softplus):
-        for t, name, dims, words in ((x, "x", (2,), "(n_frames, n_channels)"), (A, "A", (2,), "(n_channels, n_states)"),
-                                     (B, "B", (2, 3), "(n_frames, n_states) or (n_frames, n_groups, n_states)")):
-            if not isinstance(t, torch.Tensor):
-                raise ValueError(f"{name} must be a tensor on {ctx.device}")
-            if t.dim() not in dims:
-                raise ValueError(f"{name} must be {'2-D ' if dims == (2,) else ''}{words}")
+        if not (isinstance(x, torch.Tensor) and isinstance(A, torch.Tensor) and isinstance(B, torch.Tensor)
+                and x.dim() == 2 and A.dim() == 2 and B.dim() in (2, 3)):
+            self._refuse(ctx, x, A, B)
         self.code, dtype = _code(x, "x"), x.dtype
-        n, c = rows = tuple(x.shape)
+        n, c = rows = x.shape
         states = A.shape[1]
         groups = B.shape[1] if B.dim() == 3 else 1
         if groups < 1 or c % groups:
@@ -191,6 +196,15 @@ class _ScanCall:
             _rows(ctx, x, "x", rows, dtype, c), _rows(ctx, dt, "dt", rows, dtype, c),
             _rows(ctx, B, "B", wide, dtype, bc), _rows(ctx, C_, "C", wide, dtype, bc),
             0 if gate is None else _rows(ctx, gate, "gate", rows, dtype, c))
+
+    @staticmethod
+    def _refuse(ctx, x, A, B):
+        for t, name, dims, words in ((x, "x", (2,), "(n_frames, n_channels)"), (A, "A", (2,), "(n_channels, n_states)"),
+                                     (B, "B", (2, 3), "(n_frames, n_states) or (n_frames, n_groups, n_states)")):
+            if not isinstance(t, torch.Tensor):
+                raise ValueError(f"{name} must be a tensor on {ctx.device}")
+            if t.dim() not in dims:
+                raise ValueError(f"{name} must be {'2-D ' if dims == (2,) else ''}{words}")
 
 
 def selective_scan(ctx, x, dt, A, B, C, offsets=None, skip=None, gate=None, dt_bias=None, dt_softplus=True,
@@ -424,6 +438,11 @@ def _dense(t):
     return True
 
 
+def _array(kind, code, values):
+    values = array.array(code, values)
+    return (kind * len(values)).from_buffer(values)
+
+
 def _codes(tensors, name):
     try:
         return [_CODES[t.dtype] for t in tensors]
@@ -442,28 +461,31 @@ def clip_gradients(ctx, grads, max_norm, out=None):
     outs = None if out is None else list(out)
     if outs is not None and len(outs) != len(grads):
         raise ValueError(f"{len(grads)} gradients but {len(outs)} outputs")
-    device, n = ctx.device, len(grads)
+    n = len(grads)
+    # (in order: passed by one look at each property of all; else the first that is not is found)
+    even = True                                          # every tensor contiguous
     for name, tensors in (("grads", grads), ("out", outs or ())):
-        # (in order: passed by one look at each property of all; else the first that is not is found)
-        if not (all([isinstance(t, torch.Tensor) for t in tensors]) and {t.device for t in tensors} <= {device}
+        if not (set(map(type, tensors)) <= _TENSORS and set(map(torch.Tensor.get_device, tensors)) <= {_index(ctx)}
                 and not any([t.requires_grad for t in tensors])):
             for i, t in enumerate(tensors):
                 _on_device(ctx, t, f"{name}[{i}]")
-        if not all([t.is_contiguous() for t in tensors]):
+        if not all(map(torch.Tensor.is_contiguous, tensors)):
+            even = False
             for i, t in enumerate(tensors):
                 if not t.is_contiguous() and not _dense(t):
                     raise ValueError(f"{name}[{i}] must fill its memory without gaps")
-    sizes = [t.numel() for t in grads]
-    counts, tensors = (C.c_int64 * n)(*sizes), (C.c_void_p * n)(*[t.data_ptr() for t in grads])
-    dtypes = (C.c_int32 * n)(*_codes(grads, "grads"))
+    counts = _array(C.c_int64, "q", map(torch.Tensor.numel, grads))
+    tensors = _array(C.c_void_p, "Q", map(torch.Tensor.data_ptr, grads))
+    dtypes = _array(C.c_int32, "i", _codes(grads, "grads"))
     to = to_types = None
     if outs is not None:
-        for i, (t, o) in enumerate(zip(grads, outs)):
-            if o.shape != t.shape or not (o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride()):
-                raise ValueError(f"out[{i}] must have its gradient's shape and order")
-        to = (C.c_void_p * n)(*[o.data_ptr() for o in outs])
-        to_types = (C.c_int32 * n)(*_codes(outs, "out"))
-    norm = torch.empty((), dtype=torch.float64, device=device)
+        if not (even and all(map(torch.Tensor.is_same_size, grads, outs))):
+            for i, (t, o) in enumerate(zip(grads, outs)):
+                if o.shape != t.shape or not (o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride()):
+                    raise ValueError(f"out[{i}] must have its gradient's shape and order")
+        to = _array(C.c_void_p, "Q", map(torch.Tensor.data_ptr, outs))
+        to_types = _array(C.c_int32, "i", _codes(outs, "out"))
+    norm = torch.empty((), dtype=torch.float64, device=ctx.device)
     ws = _workspace(ctx, lib.srx_clip_gradients_workspace(ctx.handle, n, counts))
     check(lib.srx_clip_gradients(ctx.handle, n, tensors, counts, dtypes, to, to_types, float(max_norm),
                                  norm.data_ptr(), ws.data_ptr(), ws.numel(), ctx.stream_ptr()),
