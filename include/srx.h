@@ -376,7 +376,7 @@ int srx_mstep(srx_handle_t h, const double* stats, const srx_priors_t* priors, i
  * front-end (mfcc.py:82-96) is the fixed, centred relative of it. */
 enum srx_activation { SRX_IDENTITY = 0, SRX_SILU = 1 };
 typedef struct {
-    int32_t n_channels;
+    int32_t n_channels;     /* up to 2^24 */
     int32_t width;          /* 1 .. 8 */
     int32_t activation;
     int32_t reserved;
@@ -410,7 +410,7 @@ int srx_causal_conv_backward(srx_handle_t h, const srx_conv_t* conv, int dtype, 
  * state_in[n_utts, n_channels, n_states] (zeros if NULL); state_out (may be state_in, may be NULL) receives
  * the states behind the last frames, those of state_in for an utterance without frames. */
 typedef struct {
-    int32_t n_channels;
+    int32_t n_channels;     /* up to 2^24 */
     int32_t n_states;       /* 1 .. 64 */
     int32_t n_groups;       /* a divisor of n_channels */
     int32_t softplus;       /* 0 / 1 */
@@ -430,7 +430,8 @@ typedef struct {
     void *dx, *ddt, *dB, *dC, *dgate;
     int64_t ld_dx, ld_ddt, ld_dB, ld_dC, ld_dgate;
 } srx_scan_gradients_t;
-/* Floats of `saved`: states that a training pass keeps for srx_selective_scan_backward (every eighth frame's). */
+/* Floats of `saved`: what a training pass keeps for srx_selective_scan_backward (every eighth frame's states, and the
+ * order in which a full device takes the utterances). */
 int64_t srx_selective_scan_saved(const srx_scan_t* scan, int64_t n_utts, int64_t n_frames);
 int64_t srx_selective_scan_workspace(srx_handle_t h, const srx_scan_t* scan, int64_t n_utts, int64_t n_frames);
 /* saved: NULL, or srx_selective_scan_saved floats to fill. */
@@ -455,7 +456,7 @@ int srx_selective_scan_backward(srx_handle_t h, const srx_scan_t* scan, const sr
 
 /* Layer norm of every row: y = (x - mean) rstd weight + bias with the row's own mean and rstd =
  * 1 / sqrt(variance + eps) (variance over n, not n - 1), which are returned (mean, rstd: n_rows floats).
- * weight, bias: n_features floats, or NULL for ones and zeros.  The z-score of the front-end
+ * weight, bias: n_features (up to 2^24) floats, or NULL for ones and zeros.  The z-score of the front-end
  * (HMM_final.py:18-23) is the same along the other axis. */
 int srx_layer_norm(srx_handle_t h, const void* x, int64_t ld_x, int dtype, int64_t n_rows, int32_t n_features,
                    const float* weight, const float* bias, double eps, void* y, int64_t ld_y, float* mean,

@@ -225,6 +225,7 @@ struct DeviceGuard {
     DeviceGuard& operator=(const DeviceGuard&) = delete;
 };
 
+constexpr int kMostColumns = 1 << 24;           // values of a row, so that 32 bits count them and what lies beside them
 inline bool frame_dtype(int dtype) { return dtype == SRX_F32 || dtype == SRX_BF16 || dtype == SRX_F16; }
 
 }  // namespace srx_frames

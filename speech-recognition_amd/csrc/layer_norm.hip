@@ -422,6 +422,7 @@ int norm_run(const NormParams& p, int dtype, bool backward, hipStream_t st) {
 int check_norm(srx_handle_t h, int64_t rows, int32_t features, const char* who) {
     SRX_REQUIRE(h != nullptr, "%s: NULL context", who);
     SRX_REQUIRE(rows >= 0 && features >= 1, "%s: Shape mismatch (n_rows=%lld n_features=%d)", who, (long long)rows, features);
+    SRX_REQUIRE(features <= kMostColumns, "%s: n_features %d above 2^24", who, features);
     return SRX_OK;
 }
 

@@ -385,6 +385,7 @@ int check_conv(srx_handle_t h, const srx_conv_t* conv, int64_t utts, int64_t fra
     SRX_REQUIRE(h != nullptr, "%s: NULL context", who);
     SRX_REQUIRE(conv != nullptr, "%s: conv is NULL", who);
     SRX_REQUIRE(conv->n_channels >= 1, "%s: Shape mismatch (n_channels=%d)", who, conv->n_channels);
+    SRX_REQUIRE(conv->n_channels <= kMostColumns, "%s: n_channels %d above 2^24", who, conv->n_channels);
     SRX_REQUIRE(conv->width >= 1 && conv->width <= kConvMaxWidth, "%s: width %d outside [1, %d]", who, conv->width,
                 kConvMaxWidth);
     SRX_REQUIRE(conv->activation == SRX_IDENTITY || conv->activation == SRX_SILU, "%s: unknown activation %d", who,

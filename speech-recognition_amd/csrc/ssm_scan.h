@@ -282,7 +282,12 @@ __device__ __forceinline__ int64_t scan_slot(const ScanUnit& u, int64_t t) {
     return u.begin / kScanSaveEvery + u.utt + (t - u.begin) / kScanSaveEvery;
 }
 
-// A log2(e), so that the decay is one product and the hardware's 2^x.
+// A log2(e), so that the decay is one product and the hardware's 2^x; what is not finite becomes the largest number,
+// so that a step of zero (which the frames behind an utterance's end have) leaves a state alone, as it does for any A.
+__device__ __forceinline__ float scan_log2_decay(float a) {
+    const float v = a * 1.44269504088896341f;
+    return fabsf(v) > 3.4028234e38f ? copysignf(3.4028234e38f, v) : v;
+}
 template <int R, int S, bool Q>
 __device__ __forceinline__ void scan_load_A(const ScanParams& p, const ScanLane<R, S, Q>& w, float (&A2)[R][S]) {
 #pragma unroll
@@ -290,7 +295,7 @@ __device__ __forceinline__ void scan_load_A(const ScanParams& p, const ScanLane<
 #pragma unroll
         for (int s = 0; s < S; ++s)
             A2[r][s] = r < w.left && w.state + s < p.states
-                           ? p.A[(int64_t)(w.channel + r) * p.states + w.state + s] * 1.44269504088896341f : 0.0f;
+                           ? scan_log2_decay(p.A[(int64_t)(w.channel + r) * p.states + w.state + s]) : 0.0f;
 }
 
 // ---- forward ------------------------------------------------------------------------------
@@ -458,6 +463,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
                 for (int s = 0; s < S; ++s) {
                     b.v[s] = (float)now.b.v[s];
                     if (MODE == 0) c.v[s] = (float)now.c.v[s];
+                    if (here < TILE) b.v[s] = (w.lane >> 2) < here ? b.v[s] : 0.0f;
                 }
                 store_pack(sB + w.lane * S, b);
                 if (MODE == 0) store_pack(sC + w.lane * S, c);
@@ -555,7 +561,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanParams p
         for (int k = 0; k < 4; ++k) {
             const int r = (q * 4 + k) / S, s = w.state + (q * 4 + k) % S;
             const bool in = r < w.left && s < p.states;
-            A2[k] = in ? p.A[(int64_t)(w.channel + r) * p.states + s] * 1.44269504088896341f : 0.0f;
+            A2[k] = in ? scan_log2_decay(p.A[(int64_t)(w.channel + r) * p.states + s]) : 0.0f;
             from[k] = in && enter != nullptr ? enter[(utt * p.channels + w.channel + r) * p.states + s] : 0.0f;
             h[k] = decay[k] = 0.0f;
         }
@@ -860,6 +866,10 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                     for (int s = 0; s < S; ++s) {
                         b.v[s] = (float)now.b.v[s];
                         c.v[s] = (float)now.c.v[s];
+                        if (frames < TILE) {
+                            b.v[s] = ((w.lane & 31) >> 2) < frames ? b.v[s] : 0.0f;
+                            c.v[s] = ((w.lane & 31) >> 2) < frames ? c.v[s] : 0.0f;
+                        }
                     }
                     store_pack(sB + (w.lane & 31) * S, b);
                     store_pack(sC + (w.lane & 31) * S, c);

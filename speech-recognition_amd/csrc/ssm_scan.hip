@@ -14,6 +14,7 @@ int check_scan(srx_handle_t h, const srx_scan_t* s, int64_t utts, int64_t frames
     SRX_REQUIRE(s != nullptr, "%s: scan is NULL", who);
     SRX_REQUIRE(s->n_channels >= 1 && s->n_groups >= 1 && s->n_channels % s->n_groups == 0,
                 "%s: Shape mismatch (n_channels=%d n_groups=%d)", who, s->n_channels, s->n_groups);
+    SRX_REQUIRE(s->n_channels <= kMostColumns, "%s: n_channels %d above 2^24", who, s->n_channels);
     SRX_REQUIRE(s->n_states >= 1 && s->n_states <= 64, "%s: n_states %d outside [1, 64]", who, s->n_states);
     SRX_REQUIRE(s->A != nullptr, "%s: NULL A", who);
     SRX_REQUIRE(utts >= 0 && frames >= 0, "%s: negative size", who);

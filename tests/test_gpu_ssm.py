@@ -258,6 +258,36 @@ def test_scan_not_a_number_stays_in_its_utterance(sra, ctx):
             assert torch.equal(dirty[2][k][:21], clean[2][k][:21]) and torch.equal(dirty[2][k][39:], clean[2][k][39:]), k
 
 
+@pytest.mark.parametrize("lengths", [[5, 16, 35], [1500]])
+def test_scan_decays_without_bound_forget_at_once(sra, ctx, lengths):
+    """An A of minus infinity, or the type's lowest value, is one whose decay is 0 at any step of ordinary size: the same
+    results as with -1e30, in whole tiles and at their ends."""
+    torch = _torch()
+    rng = np.random.default_rng(27)
+    off, t, v = _scan_case(rng, lengths, 24, 16, 1, "float32")
+    dy = _draw(rng, (int(off[-1]), 24), "float32")[0]
+    got = []
+    for low in (-1e30, torch.finfo(torch.float32).min, float("-inf")):
+        A = t["A"].clone()
+        A[::3, ::2] = low
+        got.append(_run_scan(sra, ctx, off, {**t, "A": A}, dy))
+    for y, last, g in got[1:]:
+        assert torch.isfinite(y).all() and torch.equal(y, got[0][0]) and torch.equal(last, got[0][1])
+        for k in g:
+            assert torch.equal(g[k], got[0][2][k]), k
+
+
+def test_scan_infinity_in_the_last_frame_stays_infinity(sra, ctx):
+    torch = _torch()
+    rng = np.random.default_rng(28)
+    for n in (5, 16, 21):
+        off, t, v = _scan_case(rng, [n], 20, 16, 1, "float32")
+        t["B"][n - 1] = float("inf")
+        _, last = _run_scan(sra, ctx, off, t)
+        want = torch.sign(t["x"][n - 1])[:, None].expand(20, 16) * float("inf")
+        assert torch.equal(last[0], want), n
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_scan_in_pieces_by_the_caller_equals_the_whole(sra, ctx, dtype):
     """A recording that comes in three calls, its state handed on in place; then frame by frame."""

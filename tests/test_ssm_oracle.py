@@ -234,6 +234,27 @@ def test_c_entry_points_refuse_what_the_python_layer_cannot_pass():
         assert fn(*args) == _lib.SRX_EINVAL            # the new element types are the new operators' alone
 
 
+def test_sizes_beyond_what_32_bits_count_are_refused():
+    from speech_recognition_amd import _lib
+    lib, h, many = _lib.lib, _Stub().handle, 2 ** 24 + 1
+    scan = _lib.Scan(many, 3, 1, 1, 1, None, None)
+    assert lib.srx_selective_scan_workspace(h, C.byref(scan), 1, 5) == -1 and b"2^24" in lib.srx_last_error()
+    conv = _lib.Conv(many, 3, 0, 0, 1, None)
+    assert lib.srx_causal_conv_step(h, C.byref(conv), 0, None, many, 0, None, None, many, None) == _lib.SRX_EINVAL
+    assert b"2^24" in lib.srx_last_error()
+    assert lib.srx_layer_norm(h, None, many, 0, 0, many, None, None, 1e-5, None, many, None, None, None) == _lib.SRX_EINVAL
+    assert lib.srx_layer_norm_backward_workspace(h, 1, many) == -1 and b"2^24" in lib.srx_last_error()
+    # a wave reaches four rows of the channels' matrices, 16 of B and C, with 32-bit offsets
+    scan = _lib.Scan(4, 3, 1, 1, 1, None, None)
+    for rows in (_lib.ScanInputs(1, 1, 1, 1, None, 2 ** 29, 4, 3, 3, 0), _lib.ScanInputs(1, 1, 1, 1, None, 4, 2 ** 40, 3, 3, 0),
+                 _lib.ScanInputs(1, 1, 1, 1, None, 4, 4, 2 ** 27, 3, 0), _lib.ScanInputs(1, 1, 1, 1, 1, 4, 4, 3, 3, 2 ** 62)):
+        assert lib.srx_selective_scan(h, C.byref(scan), C.byref(rows), 0, 1, 1, 5, None, None, 1, 4, None, None, 0, None) \
+            == _lib.SRX_EINVAL and b"pitch" in lib.srx_last_error()
+    rows = _lib.ScanInputs(1, 1, 1, 1, None, 4, 4, 3, 3, 0)
+    assert lib.srx_selective_scan(h, C.byref(scan), C.byref(rows), 0, 1, 1, 5, None, None, 1, 2 ** 29, None, None, 0, None) \
+        == _lib.SRX_EINVAL and b"pitch" in lib.srx_last_error()
+
+
 def test_workspace_sizes_grow_with_the_problem():
     from speech_recognition_amd import _lib
     h = _Stub().handle
