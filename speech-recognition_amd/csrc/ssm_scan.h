@@ -219,9 +219,11 @@ struct ScanLane {
             if (r < left) at[r] = v.v[r];
     }
 };
-// S states of frame t of a tile's B or C from state s0 on, zeros for those that do not exist.
+// S states of frame t of a tile's B or C from state s0 on, zeros for those that do not exist and for frames behind the
+// last one.
 template <int S, typename T>
 __device__ __forceinline__ Pack<T, S> scan_load_bc(const ScanRows<T>& rows, int t, int last, int group, int s0, int states) {
+    const int there = t <= last ? states : 0;
     t = min(t, last);
     asm volatile("" : "+v"(t), "+v"(s0));
     const T* at = (const T*)(rows.at + t * rows.pitch) + (int64_t)group * states;
@@ -229,7 +231,7 @@ __device__ __forceinline__ Pack<T, S> scan_load_bc(const ScanRows<T>& rows, int 
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         const T x = at[min(s0 + s, states - 1)];
-        v.v[s] = s0 + s < states ? x : (T)0.0f;
+        v.v[s] = s0 + s < there ? x : (T)0.0f;
     }
     __builtin_amdgcn_sched_barrier(0);
     return v;
@@ -463,7 +465,6 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
                 for (int s = 0; s < S; ++s) {
                     b.v[s] = (float)now.b.v[s];
                     if (MODE == 0) c.v[s] = (float)now.c.v[s];
-                    if (here < TILE) b.v[s] = (w.lane >> 2) < here ? b.v[s] : 0.0f;
                 }
                 store_pack(sB + w.lane * S, b);
                 if (MODE == 0) store_pack(sC + w.lane * S, c);
@@ -718,13 +719,13 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
     constexpr int CH = 16 * R, NS = 4 * S, TILE = kScanSaveEvery;
     constexpr float kLn2 = 0.693147180559945309f;
     constexpr int kKept = GATE ? 6 : 4;  // 2 (x, slope of the step, gradient by the gate over the ungated output)
-    __shared__ __align__(16) float lds[kScanWaves][TILE * (6 * CH + 4 * NS) + (MODE == 0 ? 64 * (R * S + 2 * R + kKept * R) : 0)];
+    __shared__ __align__(16) float lds[kScanWaves][TILE * (5 * CH + 4 * NS) + (MODE == 0 ? 64 * (R * S + 2 * R + kKept * R) : 0)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* sD = lds[wave];               // steps
     float* sU = sD + TILE * CH;          // step times x
     float* sP = sU + TILE * CH;          // gradient of the ungated output
-    float* oU = sP + TILE * CH;          // sums over the states: dh B
-    float* oD = oU + TILE * CH;          // dh a h A
+    float* oU = sU;                      // sums over the states: dh B (in the place of what the frame has used)
+    float* oD = sP + TILE * CH;          // dh a h A
     float* oY = oD + TILE * CH;          // C h
     float* sB = oY + TILE * CH;
     float* sC = sB + TILE * NS;
@@ -866,10 +867,6 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                     for (int s = 0; s < S; ++s) {
                         b.v[s] = (float)now.b.v[s];
                         c.v[s] = (float)now.c.v[s];
-                        if (frames < TILE) {
-                            b.v[s] = ((w.lane & 31) >> 2) < frames ? b.v[s] : 0.0f;
-                            c.v[s] = ((w.lane & 31) >> 2) < frames ? c.v[s] : 0.0f;
-                        }
                     }
                     store_pack(sB + (w.lane & 31) * S, b);
                     store_pack(sC + (w.lane & 31) * S, c);
@@ -969,7 +966,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
 #pragma unroll
                         for (int s = 0; s < HALF; ++s) v.v[s] = sums[s];
                         store_pack(to_bc + j * 2 * NS, v);              // (the lanes of a row, the same values)
-                        // What the next octet needs is asked for when the last frame's registers are free.
+                        // What the next octet needs is asked for when frames' registers are free to take it.
                         if (half == 0 && k == SUB - 1 && o > 0) {
                             saved -= (int64_t)p.blocks * (R * S * 64);
                             scan_load_lanes(saved, 0, w, h0next);
