@@ -712,10 +712,11 @@ __device__ __forceinline__ void scan_sum_channels(const float (&b)[S], const flo
 }
 
 // MODE 0: the gradients.  MODE 1: only what a piece adds to the gradient of the state before it,
-// and the sum of its steps.  SUB: frames whose states and decays are held at once, 8 or 4 (then the first four
-// frames are run through once to reach the second four).
-template <typename T, int R, int S, bool GATE, int MODE, int SUB>
-__global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanParams p) {
+// and the sum of its steps.  The states and decays of eight frames are held at once; with 64 states these are more
+// registers than two waves per SIMD have, and one wave with all of them takes half the time of two that spill (64
+// utterances of 100 to 300 frames x 1536 channels, forward and backward: 3.44 ms, now 1.69).
+template <typename T, int R, int S, bool GATE, int MODE>
+__global__ __launch_bounds__(64 * kScanWaves, R * S > 8 ? 1 : 2) void scan_backward_kernel(ScanParams p) {
     constexpr int CH = 16 * R, NS = 4 * S, TILE = kScanSaveEvery;
     constexpr float kLn2 = 0.693147180559945309f;
     constexpr int kKept = GATE ? 6 : 4;  // 2 (x, slope of the step, gradient by the gate over the ungated output)
@@ -888,92 +889,69 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void scan_backward_kernel(ScanP
                     frames = TILE;
                     continue;
                 }
-                float h4[R][S];
-                if (SUB < TILE) {                                // states before the second four frames
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int s = 0; s < S; ++s) h4[r][s] = h0[r][s];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        ScanFrame<R, S> f;
-                        f.template load<true, false>(w, j, sD, sU, nullptr, sB, sC);
-#pragma unroll
-                        for (int r = 0; r < R; ++r)
-#pragma unroll
-                            for (int s = 0; s < S; ++s)
-                                h4[r][s] = fmaf(__builtin_amdgcn_exp2f(f.d.v[r] * A2[r][s]), h4[r][s], f.du.v[r] * f.b.v[s]);
-                        if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
                 float* to_bc = oBC + (w.lane >> 5) * NS + w.state + (S > 1 ? ((w.lane >> 4) & 1) * (S / 2) : 0);
-#pragma unroll 1
-                for (int half = TILE / SUB - 1; half >= 0; --half) {
-                    const int j0 = half * SUB;
-                    float a[SUB][R][S], h[SUB + 1][R][S];
+                float a[TILE][R][S], h[TILE + 1][R][S];
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int s = 0; s < S; ++s) h[0][r][s] = h0[r][s];
+#pragma unroll
+                for (int k = 0; k < TILE; ++k) {
+                    ScanFrame<R, S> f;
+                    f.template load<true, false>(w, k, sD, sU, nullptr, sB, sC);
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
-                        for (int s = 0; s < S; ++s) h[0][r][s] = SUB < TILE && half ? h4[r][s] : h0[r][s];
-#pragma unroll
-                    for (int k = 0; k < SUB; ++k) {
-                        ScanFrame<R, S> f;
-                        f.template load<true, false>(w, j0 + k, sD, sU, nullptr, sB, sC);
-#pragma unroll
-                        for (int r = 0; r < R; ++r)
-#pragma unroll
-                            for (int s = 0; s < S; ++s) {
-                                a[k][r][s] = __builtin_amdgcn_exp2f(f.d.v[r] * A2[r][s]);
-                                h[k + 1][r][s] = fmaf(a[k][r][s], h[k][r][s], f.du.v[r] * f.b.v[s]);
-                            }
-                        if (k % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-                    }
-#pragma unroll
-                    for (int k = SUB - 1; k >= 0; --k) {
-                        const int j = j0 + k;
-                        ScanFrame<R, S> f;
-                        f.template load<true, true>(w, j, sD, sU, sP, sB, sC);
-                        float db[S], dc[S];
-                        Pack<float, R> su, sd, sy;
-#pragma unroll
-                        for (int s = 0; s < S; ++s) db[s] = dc[s] = 0.0f;
-#pragma unroll
-                        for (int r = 0; r < R; ++r) {
-                            float vu = 0.0f, vd = 0.0f, vy = 0.0f;
-#pragma unroll
-                            for (int s = 0; s < S; ++s) {
-                                const float dh = fmaf(f.q.v[r], f.c.v[s], g[r][s]);
-                                dc[s] = fmaf(f.q.v[r], h[k + 1][r][s], dc[s]);
-                                if (GATE) vy = fmaf(f.c.v[s], h[k + 1][r][s], vy);
-                                db[s] = fmaf(dh, f.du.v[r], db[s]);
-                                vu = fmaf(dh, f.b.v[s], vu);
-                                g[r][s] = dh * a[k][r][s];
-                                const float m = g[r][s] * h[k][r][s];
-                                vd = fmaf(m, A2[r][s], vd);
-                                dA[r][s] = fmaf(m, f.d.v[r], dA[r][s]);
-                            }
-                            su.v[r] = quad_sum(vu);
-                            sd.v[r] = quad_sum(vd);
-                            if (GATE) sy.v[r] = quad_sum(vy);
+                        for (int s = 0; s < S; ++s) {
+                            a[k][r][s] = __builtin_amdgcn_exp2f(f.d.v[r] * A2[r][s]);
+                            h[k + 1][r][s] = fmaf(a[k][r][s], h[k][r][s], f.du.v[r] * f.b.v[s]);
                         }
-                        store_pack(oU + j * CH + w.col * R, su);        // (four lanes, the same values)
-                        store_pack(oD + j * CH + w.col * R, sd);
-                        if (GATE) store_pack(oY + j * CH + w.col * R, sy);
-                        constexpr int HALF = S > 1 ? S / 2 : 1;
-                        float sums[HALF];
-                        scan_sum_channels<S>(db, dc, sums);
-                        Pack<float, HALF> v;
+                    if (k % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                }
 #pragma unroll
-                        for (int s = 0; s < HALF; ++s) v.v[s] = sums[s];
-                        store_pack(to_bc + j * 2 * NS, v);              // (the lanes of a row, the same values)
-                        // What the next octet needs is asked for when frames' registers are free to take it.
-                        if (half == 0 && k == SUB - 1 && o > 0) {
-                            saved -= (int64_t)p.blocks * (R * S * 64);
-                            scan_load_lanes(saved, 0, w, h0next);
+                for (int k = TILE - 1; k >= 0; --k) {
+                    ScanFrame<R, S> f;
+                    f.template load<true, true>(w, k, sD, sU, sP, sB, sC);
+                    float db[S], dc[S];
+                    Pack<float, R> su, sd, sy;
+#pragma unroll
+                    for (int s = 0; s < S; ++s) db[s] = dc[s] = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        float vu = 0.0f, vd = 0.0f, vy = 0.0f;
+#pragma unroll
+                        for (int s = 0; s < S; ++s) {
+                            const float dh = fmaf(f.q.v[r], f.c.v[s], g[r][s]);
+                            dc[s] = fmaf(f.q.v[r], h[k + 1][r][s], dc[s]);
+                            if (GATE) vy = fmaf(f.c.v[s], h[k + 1][r][s], vy);
+                            db[s] = fmaf(dh, f.du.v[r], db[s]);
+                            vu = fmaf(dh, f.b.v[s], vu);
+                            g[r][s] = dh * a[k][r][s];
+                            const float m = g[r][s] * h[k][r][s];
+                            vd = fmaf(m, A2[r][s], vd);
+                            dA[r][s] = fmaf(m, f.d.v[r], dA[r][s]);
                         }
-                        if (half == 0 && k == SUB - 2 && o > 0) reader.next(p, w, TILE, next);
-                        __builtin_amdgcn_sched_barrier(0);
+                        su.v[r] = quad_sum(vu);
+                        sd.v[r] = quad_sum(vd);
+                        if (GATE) sy.v[r] = quad_sum(vy);
                     }
+                    store_pack(oU + k * CH + w.col * R, su);        // (four lanes, the same values)
+                    store_pack(oD + k * CH + w.col * R, sd);
+                    if (GATE) store_pack(oY + k * CH + w.col * R, sy);
+                    constexpr int HALF = S > 1 ? S / 2 : 1;
+                    float sums[HALF];
+                    scan_sum_channels<S>(db, dc, sums);
+                    Pack<float, HALF> v;
+#pragma unroll
+                    for (int s = 0; s < HALF; ++s) v.v[s] = sums[s];
+                    store_pack(to_bc + k * 2 * NS, v);              // (the lanes of a row, the same values)
+                    // What the next octet needs is asked for when the last frame's registers are free.
+                    if (k == TILE - 1 && o > 0) {
+                        saved -= (int64_t)p.blocks * (R * S * 64);
+                        scan_load_lanes(saved, 0, w, h0next);
+                    }
+                    if (k == TILE - 2 && o > 0) reader.next(p, w, TILE, next);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 wave_lds_fence();
                 const Pack<float, S> sums = load_pack<S>(oBC + w.lane * S);
@@ -1202,19 +1180,18 @@ int scan_forward_launch(const ScanParams& p, hipStream_t st) {
 
 template <typename T, int R, int S, bool GATE>
 int scan_backward_launch(const ScanParams& q, hipStream_t st) {
-    constexpr int SUB = R * S <= 8 ? 8 : 4;              // (what the registers of two waves per SIMD hold)
     ScanParams p = q;
     const int64_t across = (p.blocks + kScanWaves - 1) / kScanWaves;
     if (p.segment != 0) {
         const int64_t parts = p.parts;
         p.parts = p.units;
-        scan_backward_kernel<T, R, S, GATE, 1, SUB><<<scan_grid(p.units * across), 64 * kScanWaves, 0, st>>>(p);
+        scan_backward_kernel<T, R, S, GATE, 1><<<scan_grid(p.units * across), 64 * kScanWaves, 0, st>>>(p);
         SRX_HIP(hipGetLastError());
         scan_join_kernel<R, S, true><<<scan_grid(p.utts * p.blocks * (R * S / 4)), 64 * kJoinWaves, 0, st>>>(p);
         SRX_HIP(hipGetLastError());
         p.parts = parts;
     }
-    scan_backward_kernel<T, R, S, GATE, 0, SUB><<<scan_grid(p.parts * across), 64 * kScanWaves, 0, st>>>(p);
+    scan_backward_kernel<T, R, S, GATE, 0><<<scan_grid(p.parts * across), 64 * kScanWaves, 0, st>>>(p);
     SRX_HIP(hipGetLastError());
     scan_sum_parts_kernel<R, S><<<(unsigned)(p.blocks * (R * S / 4 + 1)), 256, 0, st>>>(p);
     SRX_HIP(hipGetLastError());
