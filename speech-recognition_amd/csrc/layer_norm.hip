@@ -257,16 +257,33 @@ __global__ __launch_bounds__(kSumThreads) void norm_sum_kernel(NormParams p) {
 }
 
 // Narrow rows (the front-end's features): a workgroup takes 128 of them into LDS -- as one run of memory where there
-// are no gaps between them --, each thread then has a row of its own and needs no other lane for its sums, and the
-// results leave the same way.  An odd distance between the rows in LDS keeps 64 threads on 64 banks.
-constexpr int kNarrowRows = 128, kNarrowMost = 64;
-template <typename T>
+// are no gaps between them --, each thread then has a row of its own in registers and needs no other lane for its
+// sums, and the results leave the same way.  An odd distance between the rows in LDS keeps 64 threads on 64 banks; rows of
+// an odd width lie there as in memory and are moved 16 bytes at a time.  EIGHTS: of the row's values, rounded up.
+constexpr int kNarrowRows = 128;
+
+// Calls each(element, place) for the next V elements of a run of whole rows, from element e on.
+template <int V, typename F>
+__device__ __forceinline__ void narrow_places(int e, int width, int step, const F& each) {
+    int r = e / width, c = e - r * width;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        each(v, r * step + c);
+        if (++c == width) {
+            c = 0;
+            ++r;
+        }
+    }
+}
+
+template <typename T, int EIGHTS>
 __global__ __launch_bounds__(kNarrowRows) void norm_forward_narrow_kernel(NormParams p) {
-    constexpr int V = 16 / sizeof(T);
-    extern __shared__ float rows[];              // [128][width | 1], weight and bias after them
+    constexpr int V = 16 / sizeof(T), RUN = kNarrowRows * V, AHEAD = sizeof(T), WIDE = 8 * EIGHTS;
+    extern __shared__ __align__(16) float rows[];              // [128][width | 1], weight and bias after them
     const int width = p.width, step = width | 1;
+    const bool odd = step == width;
     float* weight = rows + kNarrowRows * step;
-    float* bias = weight + width;
+    float* bias = weight + WIDE;
     for (int c = threadIdx.x; c < width; c += kNarrowRows) {
         weight[c] = p.weight != nullptr ? p.weight[c] : 1.0f;
         bias[c] = p.bias != nullptr ? p.bias[c] : 0.0f;
@@ -274,71 +291,85 @@ __global__ __launch_bounds__(kNarrowRows) void norm_forward_narrow_kernel(NormPa
     for (int64_t row0 = (int64_t)blockIdx.x * kNarrowRows; row0 < p.rows; row0 += (int64_t)gridDim.x * kNarrowRows) {
         const int here = (int)min((int64_t)kNarrowRows, p.rows - row0), count = here * width;
         __syncthreads();                         // (the last rows have left)
-        if (p.ld_x != width)
+        if (p.ld_x != width) {
             for (int e = threadIdx.x; e < count; e += kNarrowRows) {
                 const int r = e / width, c = e - r * width;
                 rows[r * step + c] = (float)((const T*)p.x)[(row0 + r) * p.ld_x + c];
             }
-        const T* x = (const T*)p.x + row0 * width;
-        for (int e = p.ld_x == width ? threadIdx.x * V : count; e < count; e += kNarrowRows * V) {
-            const Pack<T, V> in = load_where<V>(here == kNarrowRows && count % (kNarrowRows * V) == 0, x + e, count - e);
-            int r = e / width, c = e - r * width;
+        } else {
+            const T* x = (const T*)p.x + row0 * width;
+            for (int first = 0; first < count; first += AHEAD * RUN) {
+                Pack<T, V> in[AHEAD];            // (several on their way at once)
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if (e + v < count) rows[r * step + c] = (float)in.v[v];
-                if (++c == width) {
-                    c = 0;
-                    ++r;
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int e = first + k * RUN + threadIdx.x * V;
+                    in[k] = load_where<V>(first + (k + 1) * RUN <= count, x + e, count - e);
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int e = first + k * RUN + threadIdx.x * V;
+                    if (odd) {
+                        Pack<float, V> f;
+#pragma unroll
+                        for (int v = 0; v < V; ++v) f.v[v] = (float)in[k].v[v];
+                        store_where(first + (k + 1) * RUN <= count, rows + e, f, count - e);
+                    } else {
+                        narrow_places<V>(e, width, step, [&](int v, int at) {
+                            if (e + v < count) rows[at] = (float)in[k].v[v];
+                        });
+                    }
                 }
             }
         }
         __syncthreads();
         if ((int)threadIdx.x < here) {
             float* mine = rows + threadIdx.x * step;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            int c = 0;
-            for (; c + 4 <= width; c += 4)
+            float f[WIDE], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) sum[k] += mine[c + k];
-            for (; c < width; ++c) sum[c & 3] += mine[c];
+            for (int c = 0; c < WIDE; ++c) {
+                const bool in = c < WIDE - 8 || c < width;
+                f[c] = in ? mine[c] : 0.0f;
+                sum[c % 4] += f[c];
+            }
             const float mean = ((sum[0] + sum[1]) + (sum[2] + sum[3])) / (float)width;
 #pragma unroll
             for (int k = 0; k < 4; ++k) sum[k] = 0.0f;
-            for (c = 0; c + 4 <= width; c += 4)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float d = mine[c + k] - mean;
-                    sum[k] = fmaf(d, d, sum[k]);
-                }
-            for (; c < width; ++c) {
-                const float d = mine[c] - mean;
-                sum[c & 3] = fmaf(d, d, sum[c & 3]);
+            for (int c = 0; c < WIDE; ++c) {
+                f[c] = c < WIDE - 8 || c < width ? f[c] - mean : 0.0f;
+                sum[c % 4] = fmaf(f[c], f[c], sum[c % 4]);
             }
             const float rstd = 1.0f / sqrtf(((sum[0] + sum[1]) + (sum[2] + sum[3])) / (float)width + p.eps);
-#pragma unroll 4
-            for (c = 0; c < width; ++c) mine[c] = fmaf((mine[c] - mean) * rstd, weight[c], bias[c]);
+#pragma unroll
+            for (int c = 0; c < WIDE; c += 4) {
+                const Pack<float, 4> w = load_pack<4>(weight + c), b = load_pack<4>(bias + c);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (c + k < WIDE - 8 || c + k < width) mine[c + k] = fmaf(f[c + k] * rstd, w.v[k], b.v[k]);
+            }
             p.mean[row0 + threadIdx.x] = mean;
             p.rstd[row0 + threadIdx.x] = rstd;
         }
         __syncthreads();
-        if (p.ld_y != width)
+        if (p.ld_y != width) {
             for (int e = threadIdx.x; e < count; e += kNarrowRows) {
                 const int r = e / width, c = e - r * width;
                 ((T*)p.y)[(row0 + r) * p.ld_y + c] = (T)rows[r * step + c];
             }
-        T* y = (T*)p.y + row0 * width;
-        for (int e = p.ld_y == width ? threadIdx.x * V : count; e < count; e += kNarrowRows * V) {
-            int r = e / width, c = e - r * width;
-            Pack<T, V> out;
+        } else {
+            T* y = (T*)p.y + row0 * width;
+            for (int first = 0; first < count; first += RUN) {
+                const int e = first + threadIdx.x * V;
+                Pack<T, V> out;
+                if (odd) {
+                    const Pack<float, V> f = load_where<V>(first + RUN <= count, (const float*)rows + e, count - e);
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                out.v[v] = (T)(e + v < count ? rows[r * step + c] : 0.0f);
-                if (++c == width) {
-                    c = 0;
-                    ++r;
+                    for (int v = 0; v < V; ++v) out.v[v] = (T)f.v[v];
+                } else {
+                    narrow_places<V>(e, width, step, [&](int v, int at) { out.v[v] = (T)(e + v < count ? rows[at] : 0.0f); });
                 }
+                store_where(first + RUN <= count, y + e, out, count - e);
             }
-            store_where(here == kNarrowRows && count % (kNarrowRows * V) == 0, y + e, out, count - e);
         }
     }
 }
@@ -379,15 +410,31 @@ int norm_go(const NormParams& p, bool backward, hipStream_t st) {
     return SRX_OK;
 }
 
+template <typename T, int EIGHTS>
+int norm_narrow(const NormParams& p, hipStream_t st) {
+    const int64_t groups = (p.rows + kNarrowRows - 1) / kNarrowRows;
+    const size_t lds = (size_t)(kNarrowRows * (p.width | 1) + 16 * EIGHTS) * sizeof(float);
+    norm_forward_narrow_kernel<T, EIGHTS><<<(unsigned)(groups < 2 * p.parts ? groups : 2 * p.parts), kNarrowRows, lds, st>>>(p);
+    SRX_HIP(hipGetLastError());
+    return SRX_OK;
+}
+
 template <typename T>
 int norm_typed(const NormParams& p, bool backward, hipStream_t st) {
     const NormShape s = norm_shape(p.width, 4);
-    if (!backward && p.width <= kNarrowMost) {
-        const int64_t groups = (p.rows + kNarrowRows - 1) / kNarrowRows;
-        const size_t lds = (size_t)(kNarrowRows * (p.width | 1) + 2 * p.width) * sizeof(float);
-        norm_forward_narrow_kernel<T><<<(unsigned)(groups < 2 * p.parts ? groups : 2 * p.parts), kNarrowRows, lds, st>>>(p);
-        SRX_HIP(hipGetLastError());
-        return SRX_OK;
+    // Narrow rows (1,000,000 of them in float32, 16 lanes per row against one thread): 16 values 54 us and 26, 32 55 and
+    // 51, 40 67 and 78; odd widths, whose rows those lanes load value by value, 39 107 and 66, 63 137 and 111.
+    if (!backward && (p.width <= 32 || (p.width < 64 && p.width % 2 == 1))) {
+        switch ((p.width + 7) / 8) {
+            case 1: return norm_narrow<T, 1>(p, st);
+            case 2: return norm_narrow<T, 2>(p, st);
+            case 3: return norm_narrow<T, 3>(p, st);
+            case 4: return norm_narrow<T, 4>(p, st);
+            case 5: return norm_narrow<T, 5>(p, st);
+            case 6: return norm_narrow<T, 6>(p, st);
+            case 7: return norm_narrow<T, 7>(p, st);
+            default: return norm_narrow<T, 8>(p, st);
+        }
     }
     if (s.lanes == 16 && s.vectors == 1) return norm_go<T, 16, 1, 4>(p, backward, st);
     if (s.lanes == 16) return norm_go<T, 16, 2, 4>(p, backward, st);

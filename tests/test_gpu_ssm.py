@@ -480,6 +480,25 @@ def test_norm_against_oracle(sra, ctx, n, d, dtype):
         _close(db, ref["dbias"], np.abs(dyv).sum(0), n + 8, "float32", "dbias")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("n", [1, 128, 301])
+def test_norm_of_narrow_rows_without_gaps(sra, ctx, n, dtype):
+    """Rows that lie side by side travel as one run of memory: the same bits as rows with gaps, and nothing behind
+    the last one is written."""
+    torch = _torch()
+    rng = np.random.default_rng(n)
+    for d in (1, 2, 7, 8, 9, 15, 16, 23, 26, 31, 32, 33, 39, 47, 49, 55, 57, 63, 64):
+        x = _draw(rng, (n, d), dtype)[0]
+        wide = torch.zeros(n, d + 2, dtype=x.dtype, device="cuda")
+        wide[:, 1:d + 1] = x
+        w, b = (torch.from_numpy(rng.standard_normal(d).astype(np.float32)).cuda() for _ in range(2))
+        want, mean, rstd = sra.layer_norm(ctx, wide[:, 1:d + 1], w, b)
+        room = torch.full((n * d + 19,), 7.0, dtype=x.dtype, device="cuda")
+        got = sra.layer_norm(ctx, x, w, b, out=room[1:1 + n * d].view(n, d))     # (of its element's alignment only)
+        assert torch.equal(got[0], want) and torch.equal(got[1], mean) and torch.equal(got[2], rstd), d
+        assert room[0] == 7 and (room[1 + n * d:] == 7).all(), d
+
+
 def test_norm_far_from_zero_and_constant_rows(sra, ctx):
     """Rows around 1000 with a spread of one: the deviations are exact to their own size, as the mean is
     subtracted before anything is squared; a constant row gives the bias."""
