@@ -891,6 +891,8 @@ __global__ __launch_bounds__(64 * kScanWaves, R * S > 8 ? 1 : 2) void scan_backw
                 }
                 float* to_bc = oBC + (w.lane >> 5) * NS + w.state + (S > 1 ? ((w.lane >> 4) & 1) * (S / 2) : 0);
                 float a[TILE][R][S], h[TILE + 1][R][S];
+                constexpr bool kAhead = R * S <= 4;
+                ScanFrame<R, S> ahead;
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -898,7 +900,9 @@ __global__ __launch_bounds__(64 * kScanWaves, R * S > 8 ? 1 : 2) void scan_backw
 #pragma unroll
                 for (int k = 0; k < TILE; ++k) {
                     ScanFrame<R, S> f;
-                    f.template load<true, false>(w, k, sD, sU, nullptr, sB, sC);
+                    if (!kAhead || k == 0) f.template load<true, false>(w, k, sD, sU, nullptr, sB, sC);
+                    else f = ahead;
+                    if (kAhead && k + 1 < TILE) ahead.template load<true, false>(w, k + 1, sD, sU, nullptr, sB, sC);
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -911,7 +915,9 @@ __global__ __launch_bounds__(64 * kScanWaves, R * S > 8 ? 1 : 2) void scan_backw
 #pragma unroll
                 for (int k = TILE - 1; k >= 0; --k) {
                     ScanFrame<R, S> f;
-                    f.template load<true, true>(w, k, sD, sU, sP, sB, sC);
+                    if (!kAhead || k == TILE - 1) f.template load<true, true>(w, k, sD, sU, sP, sB, sC);
+                    else f = ahead;
+                    if (kAhead && k > 0) ahead.template load<true, true>(w, k - 1, sD, sU, sP, sB, sC);
                     float db[S], dc[S];
                     Pack<float, R> su, sd, sy;
 #pragma unroll
