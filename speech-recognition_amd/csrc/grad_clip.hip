@@ -265,21 +265,35 @@ int srx_clip_gradients(srx_handle_t h, int64_t n_tensors, void* const* tensors, 
     DeviceGuard guard(h->device);
     if (guard.rc) return guard.rc;
     hipStream_t st = (hipStream_t)stream;
-    const int64_t parts = need / (int64_t)sizeof(double);
-    for (int pass = 0; pass < 2; ++pass) {
+    struct Launch {
+        int64_t first, last, chunks, part;
+    };
+    std::vector<Launch> launches;
+    try {
+        launches.reserve((size_t)(n_tensors / kTensors + 1));
         int64_t part = 0;
-        rc = clip_launches(n_tensors, counts, [&](int64_t first, int64_t last, int64_t chunks) -> int {
+        clip_launches(n_tensors, counts, [&](int64_t first, int64_t last, int64_t chunks) -> int {
+            launches.push_back({first, last, chunks, part});
+            part += clip_blocks(h, chunks);
+            return SRX_OK;
+        });
+    } catch (const std::bad_alloc&) {
+        srx_set_error("%s: out of host memory", who);
+        return SRX_ENOMEM;
+    }
+    for (int pass = 0; pass < 2; ++pass) {
+        for (const Launch& l : launches) {
             ClipTable a;
             a.tensors = 0;
-            a.first_part = (int32_t)part;
-            a.parts = (int32_t)parts;
+            a.first_part = (int32_t)l.part;
+            a.parts = (int32_t)(need / (int64_t)sizeof(double));
             a.in_place = outs == nullptr;
-            a.chunks = chunks;
+            a.chunks = l.chunks;
             a.sums = (double*)workspace;
             a.norm = out_norm;
             a.max_norm = max_norm;
             int64_t at = 0;
-            for (int64_t i = first; i < last; ++i) {
+            for (int64_t i = l.first; i < l.last; ++i) {
                 if (counts[i] == 0) continue;
                 ClipTensor& t = a.t[a.tensors++];
                 t.from = tensors[i];
@@ -290,14 +304,12 @@ int srx_clip_gradients(srx_handle_t h, int64_t n_tensors, void* const* tensors, 
                 t.to_dtype = outs != nullptr ? out_dtypes[i] : dtypes[i];
                 at += clip_chunks(counts[i]);
             }
-            const int64_t blocks = clip_blocks(h, chunks);
+            const int64_t blocks = clip_blocks(h, l.chunks);
             if (pass == 0) clip_squares_kernel<<<(unsigned)blocks, kClipThreads, 0, st>>>(a);
             else clip_scale_kernel<<<(unsigned)blocks, kClipThreads, 0, st>>>(a);
             SRX_HIP(hipGetLastError());
-            part += blocks;
-            return SRX_OK;
-        });
-        if (rc) return rc;
+        }
+        std::reverse(launches.begin(), launches.end());      // (the second pass begins where the first has ended)
     }
     return SRX_OK;
 }
