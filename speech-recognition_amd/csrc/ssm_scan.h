@@ -16,6 +16,12 @@
 // gate, the loads and stores) is dealt out by rows: row g of the wave does frame 4 i + g, so that
 // nothing is computed four times either and a row's access is 16 R neighbouring channels.
 // No two waves share anything: no barriers.
+//
+// Bound by the vector ALU: per (frame, channel, state) an exponential, two products and two multiply-adds, 8 ns of a
+// SIMD per 64 of them, and about two thirds of that again for what a frame needs per channel and for LDS.  A recording
+// of 24,001 frames x 512 channels x 16 states in bfloat16 takes 113 us (24 for the recursion's arithmetic alone, 20 for
+// its bytes; cut into pieces it is computed twice), 96 utterances of 100 to 300 frames x 1024 channels in float16
+// 102 us (39, 35), forward and backward over 64 such x 1536 channels in bfloat16 406 us (122, 66).
 #pragma once
 #include "frame_ops.h"
 
