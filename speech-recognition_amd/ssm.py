@@ -225,17 +225,17 @@ def selective_scan(ctx, x, dt, A, B, C, offsets=None, skip=None, gate=None, dt_b
     utts = off.numel() - 1
     shape = (utts, a.channels, a.states)
     state = _state(ctx, state, "state", shape, torch.float32)
-    y, ld_y = _out(ctx, out, "out", (a.n, a.channels), a.dtype, a.inputs)
+    y, ld_y = _out(ctx, out, "out", (a.n, a.channels), a.dtype, (*a.inputs, *a.keep, state))
     if state_out is None:
         state_out = torch.empty(shape, dtype=torch.float32, device=ctx.device)
     else:
         _state(ctx, state_out, "state_out", shape, torch.float32)
         _apart(state_out, "state_out", *a.inputs, *a.keep, y, None if state_out is state else state)
+    ws = _workspace(ctx, lib.srx_selective_scan_workspace(ctx.handle, _ref(a.scan), utts, a.n))
     saved = None
     if save:
         saved = torch.empty((lib.srx_selective_scan_saved(_ref(a.scan), utts, a.n),), dtype=torch.float32,
                             device=ctx.device)
-    ws = _workspace(ctx, lib.srx_selective_scan_workspace(ctx.handle, _ref(a.scan), utts, a.n))
     check(lib.srx_selective_scan(ctx.handle, _ref(a.scan), _ref(a.rows), a.code, off.data_ptr(), utts, a.n,
                                  _address(state), state_out.data_ptr(), y.data_ptr(), ld_y,
                                  _address(saved), _address(ws), 0 if ws is None else ws.numel(),
@@ -259,7 +259,8 @@ def selective_scan_backward(ctx, dy, x, dt, A, B, C, offsets=None, skip=None, ga
     size = lib.srx_selective_scan_saved(_ref(a.scan), utts, a.n)
     if saved is None:
         saved = selective_scan(ctx, x, dt, A, B, C, off, skip, gate, dt_bias, dt_softplus, state, save=True)[2]
-    elif saved.dtype != torch.float32 or saved.device != ctx.device or saved.numel() != size:
+    elif not (isinstance(saved, torch.Tensor) and saved.dtype == torch.float32 and saved.device == ctx.device
+              and saved.shape == (size,) and saved.is_contiguous()):
         raise ValueError("saved must be what selective_scan(..., save=True) returned for these arguments")
 
     def like(shape, dtype=torch.float32):
@@ -295,7 +296,7 @@ def selective_scan_step(ctx, state, x, dt, A, B, C, skip=None, gate=None, dt_bia
         raise ValueError("state must be given")
     _state(ctx, state, "state", (a.n, a.channels, a.states), torch.float32)
     _apart(state, "state", *a.inputs, *a.keep)
-    y, ld_y = _out(ctx, out, "out", (a.n, a.channels), a.dtype, (*a.inputs, state))
+    y, ld_y = _out(ctx, out, "out", (a.n, a.channels), a.dtype, (*a.inputs, *a.keep, state))
     check(lib.srx_selective_scan_step(ctx.handle, _ref(a.scan), _ref(a.rows), a.code, a.n, state.data_ptr(),
                                       y.data_ptr(), ld_y, ctx.stream_ptr()),
           "srx_selective_scan_step")

@@ -163,6 +163,23 @@ def test_scan_refusals(scan_args):
     _refused("saved must be", sra.selective_scan_backward, torch.zeros(6, 4), saved=torch.zeros(3), **a)
 
 
+def test_scan_refuses_results_over_parameters_and_what_it_did_not_save(scan_args):
+    import torch
+    import speech_recognition_amd as sra
+    a = scan_args
+    room = torch.zeros(24)
+    _refused("out shares memory", sra.selective_scan, out=room.view(6, 4), state=room[:12].view(1, 4, 3), **a)
+    _refused("out shares memory", sra.selective_scan, out=room.view(6, 4), **{**a, "A": room[12:].view(4, 3)})
+    _refused("out shares memory", sra.selective_scan_step, torch.zeros(6, 4, 3), out=room.view(6, 4), skip=room[:4], **a)
+    wide = dict(a, A=torch.zeros(4, 65), B=torch.zeros(6, 65), C=torch.zeros(6, 65))
+    _refused(r"n_states 65 outside \[1, 64\]", sra.selective_scan, save=True, **wide)
+    _refused(r"n_states 65 outside \[1, 64\]", sra.selective_scan_backward, torch.zeros(6, 4), **wide)
+    from speech_recognition_amd import _lib
+    size = _lib.lib.srx_selective_scan_saved(C.byref(_lib.Scan(4, 3, 1, 1, 1, None, None)), 1, 6)
+    for saved in (torch.zeros(2 * size)[::2], torch.zeros(1, size), torch.zeros(size).double(), [0.0] * size):
+        _refused("saved must be", sra.selective_scan_backward, torch.zeros(6, 4), saved=saved, **a)
+
+
 def test_a_result_beside_its_input_in_one_matrix_is_not_refused():
     """Two halves of one projection: their memory ranges overlap, their values do not."""
     import torch
