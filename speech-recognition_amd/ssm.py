@@ -61,6 +61,9 @@ def _on_device(ctx, t, name):
 
 def _rows(ctx, t, name, shape, dtype, width):
     """Checks a matrix of rows, (n, ...) with `width` contiguous values a row; returns its pitch in elements."""
+    if (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype and t.device == ctx.device
+            and t.is_contiguous() and not t.requires_grad):
+        return width
     _on_device(ctx, t, name)
     if t.shape != shape:
         raise ValueError(f"Shape mismatch: {name} is {tuple(t.shape)}, expected {tuple(shape)}")
@@ -81,8 +84,9 @@ def _rows(ctx, t, name, shape, dtype, width):
 
 
 def _parameter(ctx, t, name, shape):
-    if t is None:
-        return None
+    if t is None or (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == torch.float32
+                     and t.device == ctx.device and t.is_contiguous() and not t.requires_grad):
+        return t
     _on_device(ctx, t, name)
     if t.shape != shape:
         raise ValueError(f"Shape mismatch: {name} is {tuple(t.shape)}, expected {tuple(shape)}")
@@ -132,7 +136,10 @@ def _apart(out, name, *inputs):
         return
     a0, a1 = _extent(out)
     for t in inputs:
-        if t is None or t.data_ptr() >= a1 or t.numel() == 0:
+        if t is None:
+            continue
+        b0 = t.data_ptr()
+        if b0 >= a1 or (t.is_contiguous() and b0 + t.nbytes <= a0) or t.numel() == 0:
             continue
         b0, b1 = _extent(t)
         if a0 >= b1:
