@@ -765,6 +765,44 @@ def test_captured_and_replayed(sra, ctx):
             assert torch.equal(a, b), rep
 
 
+def test_captured_with_offsets_that_change(sra, ctx):
+    """The offsets are the device's: a replay after they have changed is a call with the new ones, pieces, order
+    of the utterances and all; and two such calls on two streams do not meet."""
+    torch = _torch()
+    rng = np.random.default_rng(29)
+    for lengths, c in ((rng.permutation(np.arange(10, 58)), 1400), (np.array([700, 3, 0, 297]), 24)):
+        off, t, v = _scan_case(rng, lengths, c, 16, 1, "bfloat16")
+        dy = _draw(rng, (int(off[-1]), c), "bfloat16")[0]
+        o = torch.from_numpy(off).cuda()
+        args, rest = [t[k] for k in ORDER], {k: t[k] for k in REST}
+
+        def step():
+            y, last, saved = sra.selective_scan(ctx, *args, o, save=True, **rest)
+            g = sra.selective_scan_backward(ctx, dy, *args, o, saved=saved, **rest)
+            return [y, last, *g.values()]
+
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            held = step()
+        for rep in range(4):
+            o.copy_(torch.from_numpy(np.concatenate([[0], np.cumsum(rng.permutation(lengths))])))
+            graph.replay()
+            want = step()
+            torch.cuda.synchronize()
+            for k, (a, b) in enumerate(zip(held, want)):
+                assert torch.equal(a, b), (rep, k)
+        streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+        for st in streams * 2:
+            with torch.cuda.stream(st):
+                got.append(step())
+        torch.cuda.synchronize()
+        for other in got:
+            for a, b in zip(other, want):
+                assert torch.equal(a, b)
+
+
 def test_state_offsets_beyond_32_bits(sra, ctx):
     """Rows at a pitch that puts the last ones more than 2^32 bytes behind the first."""
     torch = _torch()
