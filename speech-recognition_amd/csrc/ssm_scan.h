@@ -460,6 +460,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
                         d.v[r] = 4 * i + w.row < here ? d.v[r] : 0.0f;
                         du.v[r] = 4 * i + w.row < here ? du.v[r] : 0.0f;
                     }
+                    arrive(d);                           // (a branch of the whole wave, not selections)
                 }
                 if (MODE == 1)
 #pragma unroll
@@ -517,14 +518,20 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanParam
                         }
                         out[i].v[r] = (T)v;              // the one rounding to the output's type
                     }
+                    arrive(out[i]);                      // (computed here, and not in the branch that stores it)
                 }
             }
             now = next;
             now.arrived();
             if (MODE == 0) {
+                if (here == TILE) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (4 * i + w.row < here) w.store(y, i, out[i]);
+                    for (int i = 0; i < 4; ++i) w.store(y, i, out[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (4 * i + w.row < here) w.store(y, i, out[i]);
+                }
                 y.move(TILE);
             }
         }
