@@ -1064,10 +1064,10 @@ __global__ __launch_bounds__(64 * kScanWaves, R * S > 8 ? 1 : 2) void scan_backw
 // dA, dskip, dbias: the parts of a channel block added up, always in the same order.  Workgroup (block, k):
 // k < R S / 4: quads k of dA; k == R S / 4: the two vectors.  Wave w takes every fourth part.
 template <int R, int S>
-__global__ __launch_bounds__(256) void scan_sum_parts_kernel(ScanParams p) {
+__device__ __forceinline__ void scan_sum_parts(const ScanParams& p, int task) {
     constexpr int CH = 16 * R, QUADS = R * S / 4;
     __shared__ double sum[4][64][4];
-    const int block = blockIdx.x / (QUADS + 1), k = blockIdx.x % (QUADS + 1);
+    const int block = task / (QUADS + 1), k = task % (QUADS + 1);
     const int wave = threadIdx.x >> 6;
     const ScanLane<R, S, false> w(p, block);
     double v[4] = {0.0, 0.0, 0.0, 0.0};
@@ -1106,12 +1106,12 @@ __global__ __launch_bounds__(256) void scan_sum_parts_kernel(ScanParams p) {
 
 // dB, dC: the channel blocks of a group added up.  One thread per frame, group, B or C, and state.
 template <typename T, int S>
-__global__ __launch_bounds__(256) void scan_sum_bc_kernel(ScanParams p) {
+__device__ __forceinline__ void scan_sum_bc(const ScanParams& p, int64_t group, int64_t groups) {
     constexpr int NS = 4 * S;
     const int64_t first = min(max(p.off[0], (int64_t)0), p.frames);
     const int64_t last = min(max(p.off[p.utts], first), p.frames);
     const int64_t total = (last - first) * p.groups * 2 * NS;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    for (int64_t i = group * 256 + threadIdx.x; i < total; i += groups * 256) {
         const int e = (int)(i % (2 * NS)), state = e % NS;
         const int64_t rest = i / (2 * NS);
         const int g = (int)(rest % p.groups);
@@ -1133,6 +1133,14 @@ __global__ __launch_bounds__(256) void scan_sum_bc_kernel(ScanParams p) {
             else ((T*)p.dC)[t * p.ld_dC + at] = (T)v;
         }
     }
+}
+
+// Both in one launch: the first workgroups take the parameters' parts, the others dB and dC.
+template <typename T, int R, int S>
+__global__ __launch_bounds__(256) void scan_sum_kernel(ScanParams p) {
+    const unsigned parts = (unsigned)p.blocks * (R * S / 4 + 1);
+    if (blockIdx.x < parts) scan_sum_parts<R, S>(p, (int)blockIdx.x);
+    else scan_sum_bc<T, S>(p, blockIdx.x - parts, gridDim.x - parts);
 }
 
 // ---- one frame of every stream --------------------------------------------------------------
@@ -1219,13 +1227,10 @@ int scan_backward_launch(const ScanParams& q, hipStream_t st) {
     }
     scan_backward_kernel<T, R, S, GATE, 0><<<scan_grid(p.parts * across), 64 * kScanWaves, 0, st>>>(p);
     SRX_HIP(hipGetLastError());
-    scan_sum_parts_kernel<R, S><<<(unsigned)(p.blocks * (R * S / 4 + 1)), 256, 0, st>>>(p);
-    SRX_HIP(hipGetLastError());
     const int64_t sums = p.utts > 0 ? p.frames * p.groups * 8 * S : 0;
-    if (sums > 0) {
-        scan_sum_bc_kernel<T, S><<<scan_grid((sums + 255) / 256), 256, 0, st>>>(p);
-        SRX_HIP(hipGetLastError());
-    }
+    const unsigned wide = sums > 0 ? scan_grid((sums + 255) / 256) : 0;
+    scan_sum_kernel<T, R, S><<<(unsigned)(p.blocks * (R * S / 4 + 1)) + wide, 256, 0, st>>>(p);
+    SRX_HIP(hipGetLastError());
     return SRX_OK;
 }
 
