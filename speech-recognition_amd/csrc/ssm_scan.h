@@ -19,9 +19,9 @@
 //
 // Bound by the vector ALU: per (frame, channel, state) an exponential, two products and two multiply-adds, 9 ns of a
 // SIMD per 64 of them, and about two thirds of that again for what a frame needs per channel and for LDS.  A recording
-// of 24,001 frames x 512 channels x 16 states in bfloat16 takes 113 us (28 for the recursion's arithmetic alone, 20 for
+// of 24,001 frames x 512 channels x 16 states in bfloat16 takes 112 us (28 for the recursion's arithmetic alone, 20 for
 // its bytes; cut into pieces it is computed twice), 96 utterances of 100 to 300 frames x 1024 channels in float16
-// 102 us (44, 35), forward and backward over 64 such x 1536 channels in bfloat16 406 us (124, 66).  One channel per lane
+// 102 us (44, 35), forward and backward over 64 such x 1536 channels in bfloat16 401 us (124, 66).  One channel per lane
 // with all its states, which needs no sums across lanes and no LDS but for B and C, has 8 % fewer instructions but
 // registers for two waves per SIMD only, and is slower (124, 142).
 #pragma once
