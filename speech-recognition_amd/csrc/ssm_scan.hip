@@ -58,7 +58,8 @@ ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, i
     const int64_t simds = (int64_t)h->n_cu * 4;
     auto blocks_of = [&](int wide) { return (int64_t)s->n_groups * ((p.per_group + 16 * wide - 1) / (16 * wide)); };
     // Two channels a lane, or one where two leave too few waves (the work beside the exponentials is smaller for
-    // two) and from 17 states on, whose registers leave no room for more.
+    // two) and from 17 states on, whose registers leave no room for more.  Utterances of 200 frames x 1024 channels, 16
+    // states, forward and backward: 32 of them 173 us with two and 158 with one, 64 of them 261 and 300.
     p.wide = s->n_states <= 4 ? 4 : 2;
     if (s->n_states > 16 || (s->n_states > 8 && utts * blocks_of(2) < 2 * simds)) p.wide = 1;
     p.group_blocks = (p.per_group + 16 * p.wide - 1) / (16 * p.wide);
