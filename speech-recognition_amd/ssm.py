@@ -154,12 +154,16 @@ def _apart(out, name, *inputs):
 
 
 def _out(ctx, out, name, shape, dtype, inputs):
-    """(the result's tensor, its pitch in elements); the first input has its type"""
+    """(the result's tensor, its pitch in elements); the first input has its type and shape"""
     if out is None:
-        return inputs[0].new_empty(shape), shape[1]
+        return _like(inputs[0]), shape[1]
     pitch = _rows(ctx, out, name, shape, dtype, shape[1])
     _apart(out, name, *inputs)
     return out, pitch
+
+
+def _like(t):
+    return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _address(t):
@@ -270,16 +274,8 @@ def selective_scan_backward(ctx, dy, x, dt, A, B, C, offsets=None, skip=None, ga
               and saved.shape == (size,) and saved.is_contiguous()):
         raise ValueError("saved must be what selective_scan(..., save=True) returned for these arguments")
 
-    def like(shape, dtype=torch.float32):
-        return torch.empty(shape, dtype=dtype, device=ctx.device)
-
-    rows = (a.n, a.channels)
-    grads = {"x": like(rows, a.dtype), "dt": like(rows, a.dtype), "A": like((a.channels, a.states)),
-             "B": like(a.wide, a.dtype), "C": like(a.wide, a.dtype),
-             "skip": None if skip is None else like((a.channels,)),
-             "gate": None if gate is None else like(rows, a.dtype),
-             "dt_bias": None if dt_bias is None else like((a.channels,)),
-             "state": None if state is None else like(shape)}
+    grads = {"x": _like(x), "dt": _like(dt), "A": _like(A), "B": _like(B), "C": _like(C), "skip": _like(skip),
+             "gate": _like(gate), "dt_bias": _like(dt_bias), "state": _like(state)}
     bc = a.groups * a.states
     to = _lib.ScanGradients(grads["x"].data_ptr(), grads["dt"].data_ptr(), grads["B"].data_ptr(),
                             grads["C"].data_ptr(), _address(grads["gate"]), a.channels, a.channels, bc, bc,
@@ -366,10 +362,7 @@ def causal_conv_backward(ctx, dy, x, weight, offsets=None, bias=None, activation
     state = _state(ctx, state, "state", shape, x.dtype)
     dstate_out = _state(ctx, dstate_out, "dstate_out", shape, x.dtype)
     ld_dy = _rows(ctx, dy, "dy", (a.n, a.channels), x.dtype, a.channels)
-    grads = {"x": torch.empty((a.n, a.channels), dtype=x.dtype, device=ctx.device),
-             "weight": torch.empty((a.channels, a.width), dtype=torch.float32, device=ctx.device),
-             "bias": None if bias is None else torch.empty((a.channels,), dtype=torch.float32, device=ctx.device),
-             "state": None if state is None else torch.empty(shape, dtype=x.dtype, device=ctx.device)}
+    grads = {"x": _like(x), "weight": _like(weight), "bias": _like(bias), "state": _like(state)}
     ws = _workspace(ctx, lib.srx_causal_conv_backward_workspace(ctx.handle, _ref(a.conv), utts, a.n))
     check(lib.srx_causal_conv_backward(ctx.handle, _ref(a.conv), a.code, x.data_ptr(), a.ld, off.data_ptr(), utts,
                                        a.n, _address(state), dy.data_ptr(), ld_dy, _address(dstate_out),
@@ -421,7 +414,7 @@ def layer_norm_backward(ctx, dy, x, mean, rstd, weight=None):
     ld_dy = _rows(ctx, dy, "dy", rows, x.dtype, d)
     mean, rstd = _parameter(ctx, mean, "mean", (n,)), _parameter(ctx, rstd, "rstd", (n,))
     weight = _parameter(ctx, weight, "weight", (d,))
-    dx = torch.empty((n, d), dtype=x.dtype, device=ctx.device)
+    dx = _like(x)
     dweight = torch.empty((d,), dtype=torch.float32, device=ctx.device)
     dbias = torch.empty((d,), dtype=torch.float32, device=ctx.device)
     ws = _workspace(ctx, lib.srx_layer_norm_backward_workspace(ctx.handle, n, d))
