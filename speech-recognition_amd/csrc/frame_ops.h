@@ -84,13 +84,14 @@ __device__ __forceinline__ void store_where(bool all, T* p, const Pack<T, V>& v,
 }
 
 // e^x by the hardware's 2^x; the part of x log2(e) that its rounding to 32 bits drops is put
-// back to first order, so that the relative error does not grow with |x|.
+// back to first order, so that the relative error does not grow with |x|.  0 and infinity stay as they are: they have no
+// such error, and where the product itself overflows there is no dropped part (it would come out as NaN).
 __device__ __forceinline__ float exp_f32(float x) {
     const float kLog2e = 1.44269504088896341f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147180559945309f;
     const float t = x * kLog2e;
     const float rest = fmaf(x, kLog2e, -t) + x * kLog2eRest;
     const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, rest * kLn2, e);
+    return e > 0.0f && e < __builtin_huge_valf() ? fmaf(e, rest * kLn2, e) : e;
 }
 __device__ __forceinline__ float sigmoid_f32(float x) {
     // (the exponential overflows to infinity for x below -88, the quotient is then zero)

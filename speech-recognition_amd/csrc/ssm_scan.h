@@ -292,12 +292,11 @@ __device__ __forceinline__ int64_t scan_slot(const ScanUnit& u, int64_t t) {
     return u.begin / kScanSaveEvery + u.utt + (t - u.begin) / kScanSaveEvery;
 }
 
-// A log2(e), so that the decay is one product and the hardware's 2^x; what is not finite becomes the largest number,
-// so that a step of zero (which the frames behind an utterance's end have) leaves a state alone, as it does for any A.
-__device__ __forceinline__ float scan_log2_decay(float a) {
-    const float v = a * 1.44269504088896341f;
-    return fabsf(v) > 3.4028234e38f ? copysignf(3.4028234e38f, v) : v;
-}
+// An infinite rate of decay becomes the largest number, so that a step of zero (which the frames behind an utterance's
+// end have) leaves a state alone, as it does for any A.
+__device__ __forceinline__ float scan_finite(float v) { return fabsf(v) > 3.4028234e38f ? copysignf(3.4028234e38f, v) : v; }
+// A log2(e), so that the decay is one product and the hardware's 2^x.
+__device__ __forceinline__ float scan_log2_decay(float a) { return scan_finite(a * 1.44269504088896341f); }
 template <int R, int S, bool Q>
 __device__ __forceinline__ void scan_load_A(const ScanParams& p, const ScanLane<R, S, Q>& w, float (&A2)[R][S]) {
 #pragma unroll
@@ -1171,7 +1170,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanParams p, float* sta
             const Pack<T, 4> q = load_some<4>((const T*)p.C + row * p.ld_C + bc + n0, left);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                v.v[k] = fmaf(exp_f32(d * a.v[k]), v.v[k], du * (float)b.v[k]);
+                v.v[k] = fmaf(exp_f32(d * scan_finite(a.v[k])), v.v[k], du * (float)b.v[k]);
                 y = fmaf((float)q.v[k], v.v[k], y);
             }
             store_some(h + n0, v, left);

@@ -819,3 +819,51 @@ def test_state_offsets_beyond_32_bits(sra, ctx):
     a, b = sra.causal_conv(ctx, t["x"], w), sra.causal_conv(ctx, far, w)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     assert torch.equal(sra.layer_norm(ctx, t["x"])[0], sra.layer_norm(ctx, far)[0])
+
+
+# ---- values without bound, in the single-frame form, in padded states and channels, behind a last frame ----------------
+
+@pytest.mark.parametrize("low", [-3e38, -3.4028234663852886e38, float("-inf")])
+def test_scan_step_decays_without_bound_forget_at_once(sra, ctx, low):
+    """The single frame as the recording: a decay without bound is 0, the same results as with -1e30 (whose decay is 0
+    at steps above 1e-28, and these are above e^-10); a step of 0, whatever A is, leaves the state as it was."""
+    torch = _torch()
+    rng = np.random.default_rng(30)
+    off, t, v = _scan_case(rng, [1] * 6, 20, 16, 1, "float32")
+    t["dt"][4], v["dt"][4] = float("-inf"), -np.inf
+    got = []
+    for a in (-1e30, low):
+        A, state = t["A"].clone(), t["state"].clone()
+        A[::3, ::2] = a
+        y = sra.selective_scan_step(ctx, state, t["x"], t["dt"], A, t["B"], t["C"], skip=t["skip"], gate=t["gate"],
+                                    dt_bias=t["dt_bias"])
+        got.append((y, state))
+    v["A"][::3, ::2] = -1e30
+    args = {q: v[q] for q in (*ORDER, *REST)}
+    ref, size = so.scan(off, **args), so.scan(off, scales=True, **args)
+    _close(got[0][0], ref["y"], size["y"], 4 + 2 * 16 + 40, "float32", "y")
+    _close(got[0][1], ref["state_out"], size["state_out"], 4 + 2 * 16 + 40, "float32", "state")
+    assert torch.equal(got[1][0], got[0][0]) and torch.equal(got[1][1], got[0][1])
+    assert torch.equal(got[1][1][4], t["state"][4])
+    # a recording handed from one form to the other
+    A = t["A"].clone()
+    A[::3, ::2] = low
+    state = _run_scan(sra, ctx, off, {**t, "A": A})[1]
+    y = sra.selective_scan_step(ctx, state, t["x"], t["dt"], A, t["B"], t["C"], dt_bias=t["dt_bias"])
+    assert torch.isfinite(y).all() and torch.isfinite(state).all()
+
+
+@pytest.mark.parametrize("high", [89.0, 1000.0, 3.4028234663852886e38, float("inf")])
+def test_scan_step_growth_without_bound_is_infinity(sra, ctx, high):
+    """e^89 and more is infinity in 32 bits: infinite states of the old ones' signs, in both forms."""
+    torch = _torch()
+    rng = np.random.default_rng(31)
+    off, t, v = _scan_case(rng, [1] * 3, 20, 16, 1, "float32")
+    t["dt"] = torch.ones_like(t["dt"])
+    t["A"] = torch.full_like(t["A"], high)
+    args = [t["x"], t["dt"], t["A"], t["B"], t["C"]]
+    want = torch.sign(t["state"]) * float("inf")
+    _, last = sra.selective_scan(ctx, *args, torch.arange(4, device="cuda"), state=t["state"], dt_softplus=False)
+    state = t["state"].clone()
+    sra.selective_scan_step(ctx, state, *args, dt_softplus=False)
+    assert torch.equal(last, want) and torch.equal(state, want)
