@@ -933,43 +933,53 @@ __global__ __launch_bounds__(64 * kScanWaves, R * S > 8 ? 1 : 2) void scan_backw
                 }
 #pragma unroll
                 for (int k = TILE - 1; k >= 0; --k) {
+                    // A frame behind the utterance's last adds nothing to dA, but its zeros would, times an infinite
+                    // state.  It is passed by, or left out of that sum alone where the next frame's values are read ahead
+                    // (64 utterances of 100 to 300 frames x 1024 channels, forward and backward, 7 states: 255 us and 249;
+                    // 16 states in float32 with a gate 304 and 321).
+                    const bool live = k == 0 || k < frames;
                     ScanFrame<R, S> f;
-                    if (!kAhead || k == TILE - 1) f.template load<true, true>(w, k, sD, sU, sP, sB, sC);
-                    else f = ahead;
-                    if (kAhead && k > 0) ahead.template load<true, true>(w, k - 1, sD, sU, sP, sB, sC);
-                    float db[S], dc[S];
-                    Pack<float, R> su, sd, sy;
-#pragma unroll
-                    for (int s = 0; s < S; ++s) db[s] = dc[s] = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        float vu = 0.0f, vd = 0.0f, vy = 0.0f;
-#pragma unroll
-                        for (int s = 0; s < S; ++s) {
-                            const float dh = fmaf(f.q.v[r], f.c.v[s], g[r][s]);
-                            dc[s] = fmaf(f.q.v[r], h[k + 1][r][s], dc[s]);
-                            if (GATE) vy = fmaf(f.c.v[s], h[k + 1][r][s], vy);
-                            db[s] = fmaf(dh, f.du.v[r], db[s]);
-                            vu = fmaf(dh, f.b.v[s], vu);
-                            g[r][s] = dh * a[k][r][s];
-                            const float m = g[r][s] * h[k][r][s];
-                            vd = fmaf(m, A2[r][s], vd);
-                            dA[r][s] = fmaf(m, f.d.v[r], dA[r][s]);
-                        }
-                        su.v[r] = quad_sum(vu);
-                        sd.v[r] = quad_sum(vd);
-                        if (GATE) sy.v[r] = quad_sum(vy);
+                    if (kAhead) {
+                        if (k == TILE - 1) f.template load<true, true>(w, k, sD, sU, sP, sB, sC);
+                        else f = ahead;
+                        if (k > 0) ahead.template load<true, true>(w, k - 1, sD, sU, sP, sB, sC);
                     }
-                    store_pack(oU + k * CH + w.col * R, su);        // (four lanes, the same values)
-                    store_pack(oD + k * CH + w.col * R, sd);
-                    if (GATE) store_pack(oY + k * CH + w.col * R, sy);
-                    constexpr int HALF = S > 1 ? S / 2 : 1;
-                    float sums[HALF];
-                    scan_sum_channels<S>(db, dc, sums);
-                    Pack<float, HALF> v;
+                    if (kAhead || live) {
+                        if (!kAhead) f.template load<true, true>(w, k, sD, sU, sP, sB, sC);
+                        float db[S], dc[S];
+                        Pack<float, R> su, sd, sy;
 #pragma unroll
-                    for (int s = 0; s < HALF; ++s) v.v[s] = sums[s];
-                    store_pack(to_bc + k * 2 * NS, v);              // (the lanes of a row, the same values)
+                        for (int s = 0; s < S; ++s) db[s] = dc[s] = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            float vu = 0.0f, vd = 0.0f, vy = 0.0f;
+#pragma unroll
+                            for (int s = 0; s < S; ++s) {
+                                const float dh = fmaf(f.q.v[r], f.c.v[s], g[r][s]);
+                                dc[s] = fmaf(f.q.v[r], h[k + 1][r][s], dc[s]);
+                                if (GATE) vy = fmaf(f.c.v[s], h[k + 1][r][s], vy);
+                                db[s] = fmaf(dh, f.du.v[r], db[s]);
+                                vu = fmaf(dh, f.b.v[s], vu);
+                                g[r][s] = dh * a[k][r][s];
+                                const float m = g[r][s] * h[k][r][s];
+                                vd = fmaf(m, A2[r][s], vd);
+                                dA[r][s] = !kAhead || live ? fmaf(m, f.d.v[r], dA[r][s]) : dA[r][s];
+                            }
+                            su.v[r] = quad_sum(vu);
+                            sd.v[r] = quad_sum(vd);
+                            if (GATE) sy.v[r] = quad_sum(vy);
+                        }
+                        store_pack(oU + k * CH + w.col * R, su);        // (four lanes, the same values)
+                        store_pack(oD + k * CH + w.col * R, sd);
+                        if (GATE) store_pack(oY + k * CH + w.col * R, sy);
+                        constexpr int HALF = S > 1 ? S / 2 : 1;
+                        float sums[HALF];
+                        scan_sum_channels<S>(db, dc, sums);
+                        Pack<float, HALF> v;
+#pragma unroll
+                        for (int s = 0; s < HALF; ++s) v.v[s] = sums[s];
+                        store_pack(to_bc + k * 2 * NS, v);              // (the lanes of a row, the same values)
+                    }
                     // What the next octet needs is asked for when the last frame's registers are free.
                     if (k == TILE - 1 && o > 0) {
                         saved -= (int64_t)p.blocks * (R * S * 64);

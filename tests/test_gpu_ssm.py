@@ -867,3 +867,34 @@ def test_scan_step_growth_without_bound_is_infinity(sra, ctx, high):
     state = t["state"].clone()
     sra.selective_scan_step(ctx, state, *args, dt_softplus=False)
     assert torch.equal(last, want) and torch.equal(state, want)
+
+
+def _same(got, ref, size, k, dtype, what):
+    """Like _close where the definition is finite, of infinities the signs; what it leaves open (NaN) is not compared."""
+    got, far = _host(got), np.isinf(ref)
+    assert np.array_equal(got[far], ref[far]), f"{what}: {(got[far] != ref[far]).sum()} of {far.sum()} infinities differ"
+    keep = np.isfinite(ref)
+    assert np.isfinite(got[keep]).all(), f"{what}: {(~np.isfinite(got[keep])).sum()} of {keep.sum()} are not finite"
+    _close(_torch().from_numpy(got[keep]), ref[keep], size[keep], k, dtype, what)
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("lengths,c,s", [([5], 20, 16), ([8, 13], 20, 16), ([1, 3, 16, 22], 40, 8), ([19], 70, 4), ([300], 24, 16),
+                                         ([9, 7], 17, 24), ([12], 16, 64)])
+def test_scan_infinity_in_a_last_frame_spares_the_gradients_before_it(sra, ctx, lengths, c, s):
+    """An infinite state behind the last frame is no factor of any gradient but that frame's own: what the frames of
+    an octet behind the end add to dA is nothing."""
+    torch = _torch()
+    rng = np.random.default_rng(32)
+    off, t, v = _scan_case(rng, lengths, c, s, 1, "float32")
+    dy, dyv = _draw(rng, (off[-1], c), "float32")
+    dsov = rng.standard_normal((len(lengths), c, s)).astype(np.float32)
+    for end in off[1:]:
+        t["B"][end - 1], v["B"][end - 1] = float("inf"), np.inf
+    args = {**{q: v[q] for q in (*ORDER, *REST)}, "dy": dyv, "dstate_out": dsov.astype(np.float64)}
+    ref, size = so.scan(off, **args), so.scan(off, scales=True, **args)
+    grads = _run_scan(sra, ctx, off, t, dy, torch.from_numpy(dsov).cuda())[2]
+    assert np.isfinite(ref["dA"]).all() and np.isfinite(ref["dskip"]).all() and np.isfinite(ref["dstate"]).all()
+    kb = 2 * (4 * max(lengths) + 2 * s + 40) + c + 64
+    for q in ("A", "skip", "state", "B"):
+        _same(grads[q], ref["d" + q], size["d" + q], kb + (off[-1] if q != "B" else 0), "float32", "d" + q)
