@@ -562,6 +562,11 @@ __global__ __launch_bounds__(64 * kScanWaves, R < 4 && R * S <= 8 ? 4 : 1) void 
 // walk over their run again with the state that enters it.
 // (Few pieces keep few waves busy: with seven of them a workgroup of 4 takes 4.7 us and one of 16 6.6, with 125 19.8 and
 // 11.6.)
+// A state that is zero stays zero, though its growth over all of a piece (an A above zero, or steps below) may be beyond 32
+// bits while that of every frame is not.
+__device__ __forceinline__ float scan_join(float log2_decay, float h, float own) {
+    return fmaf(h != 0.0f ? __builtin_amdgcn_exp2f(log2_decay) : 0.0f, h, own);
+}
 constexpr int kJoinWaves = 16;
 inline int scan_join_threads(const ScanParams& p) { return 64 * (p.frames / (p.segment * p.utts) < 16 ? 4 : kJoinWaves); }
 template <int R, int S, bool REVERSE>
@@ -614,7 +619,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanParams p
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        h[e] = fmaf(__builtin_amdgcn_exp2f(sum[a][e] * A2[e]), h[e], own[a].v[e]);
+                        h[e] = scan_join(sum[a][e] * A2[e], h[e], own[a].v[e]);
                         decay[e] += sum[a][e];
                     }
                 }
@@ -631,7 +636,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanParams p
         for (int before = 0; before < wave; ++before)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                h[e] = fmaf(__builtin_amdgcn_exp2f(lds[before][1][w.lane][e] * A2[e]), h[e], lds[before][0][w.lane][e]);
+                h[e] = scan_join(lds[before][1][w.lane][e] * A2[e], h[e], lds[before][0][w.lane][e]);
         walk(true);
         __syncthreads();                                 // (the next task's results go to the same place)
     }

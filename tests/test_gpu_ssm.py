@@ -898,3 +898,28 @@ def test_scan_infinity_in_a_last_frame_spares_the_gradients_before_it(sra, ctx, 
     kb = 2 * (4 * max(lengths) + 2 * s + 40) + c + 64
     for q in ("A", "skip", "state", "B"):
         _same(grads[q], ref["d" + q], size["d" + q], kb + (off[-1] if q != "B" else 0), "float32", "d" + q)
+
+
+@pytest.mark.parametrize("s", [3, 16])
+def test_scan_in_pieces_that_begin_with_silence_and_grow(sra, ctx, s):
+    """A state that is zero stays zero however much a piece would let it grow (e^32 and more per piece, beyond 32 bits
+    over a few of them), forwards and for the gradients backwards.  A decay of e^1 is off by its exponent's two roundings
+    and its own, less than 4 E, which the 4 L of the tolerance has."""
+    torch = _torch()
+    rng = np.random.default_rng(33)
+    off, t, v = _scan_case(rng, [400], 24, s, 1, "float32", state=False, bias=False)
+    t["dt"], v["dt"] = torch.ones_like(t["dt"]), np.ones_like(v["dt"])
+    t["A"], v["A"] = torch.ones_like(t["A"]), np.ones_like(v["A"])
+    t["x"][:380], v["x"][:380] = 0, 0
+    dy, dyv = _draw(rng, (400, 24), "float32")
+    dy[20:], dyv[20:] = 0, 0
+    args = {**{q: v[q] for q in (*ORDER, *REST)}, "dy": dyv, "dt_softplus": False}
+    ref, size = so.scan(off, **args), so.scan(off, scales=True, **args)
+    y, last, grads = _run_scan(sra, ctx, off, t, dy, softplus=False)
+    k = 4 * 400 + 2 * s + 40
+    assert not y[:380].any()
+    _close(y, ref["y"], size["y"], k, "float32", "y")
+    _close(last, ref["state_out"], size["state_out"], k, "float32", "state_out")
+    for q, grad in grads.items():
+        if grad is not None:
+            _close(grad, ref["d" + q], size["d" + q], 2 * k + 24 + 64 + 400, "float32", "d" + q)
