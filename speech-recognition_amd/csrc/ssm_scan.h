@@ -562,10 +562,12 @@ __global__ __launch_bounds__(64 * kScanWaves, R < 4 && R * S <= 8 ? 4 : 1) void 
 // walk over their run again with the state that enters it.
 // (Few pieces keep few waves busy: with seven of them a workgroup of 4 takes 4.7 us and one of 16 6.6, with 125 19.8 and
 // 11.6.)
-// A state that is zero stays zero, though its growth over all of a piece (an A above zero, or steps below) may be beyond 32
-// bits while that of every frame is not.
+// A state that is zero stays zero, and an infinite one infinite, as they do over the piece's frames one after the other:
+// the growth over all of a piece (an A above zero, or steps below) may be beyond 32 bits while that of every frame is not,
+// and its decay may be 0.
 __device__ __forceinline__ float scan_join(float log2_decay, float h, float own) {
-    return fmaf(h != 0.0f ? __builtin_amdgcn_exp2f(log2_decay) : 0.0f, h, own);
+    const bool scaled = h != 0.0f && fabsf(h) < __builtin_huge_valf();
+    return fmaf(scaled ? __builtin_amdgcn_exp2f(log2_decay) : 1.0f, h, own);
 }
 constexpr int kJoinWaves = 16;
 inline int scan_join_threads(const ScanParams& p) { return 64 * (p.frames / (p.segment * p.utts) < 16 ? 4 : kJoinWaves); }

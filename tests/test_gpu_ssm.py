@@ -923,3 +923,35 @@ def test_scan_in_pieces_that_begin_with_silence_and_grow(sra, ctx, s):
     for q, grad in grads.items():
         if grad is not None:
             _close(grad, ref["d" + q], size["d" + q], 2 * k + 24 + 64 + 400, "float32", "d" + q)
+
+
+def _check_infinity(sra, ctx, off, t, v, dtype, rng, which):
+    """Forward and backward with an infinity in the last utterance, in the last channel or group, all else positive."""
+    n, c = v["x"].shape
+    longest = int(np.diff(off).max())
+    for k in ("x", "B", "C", "gate", "skip"):
+        t[k], v[k] = t[k].abs(), np.abs(v[k])
+    dy, dyv = _draw(rng, (n, c), dtype)
+    dy, dyv = dy.abs(), np.abs(dyv)
+    for q in ({**t, "dy": dy}, {**v, "dy": dyv}):
+        q[which][n - int(off[-1] - off[-2]) // 2 - 2, -1] = float("inf")
+    args = {q: v[q] for q in (*ORDER, *REST)}
+    ref, size = so.scan(off, dy=dyv, **args), so.scan(off, dy=dyv, scales=True, **args)
+    got = _run_scan(sra, ctx, off, t, dy)
+    k = 4 * longest + 2 * v["A"].shape[1] + 40
+    _same(got[0], ref["y"], size["y"], k, dtype, "y")
+    _same(got[1], ref["state_out"], size["state_out"], k, "float32", "state_out")
+    for q, grad in got[2].items():
+        if grad is not None:
+            param = q in ("A", "skip", "dt_bias")
+            _same(grad, ref["d" + q], size["d" + q], 2 * k + c + 64 + (n if param else 0), "float32" if param else dtype, "d" + q)
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("which", ["x", "dy"])
+@pytest.mark.parametrize("lengths,c,s", [([300], 32, 16), ([704], 64, 4), ([129, 304], 16, 32)])
+def test_scan_infinities_pass_from_piece_to_piece(sra, ctx, lengths, c, s, which):
+    """Where the decay over a piece is 0 in 32 bits, that of every frame is not: infinity stays."""
+    rng = np.random.default_rng(38)
+    off, t, v = _scan_case(rng, lengths, c, s, 1, "float32", state=False)
+    _check_infinity(sra, ctx, off, t, v, "float32", rng, which)
