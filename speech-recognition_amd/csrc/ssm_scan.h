@@ -202,6 +202,7 @@ struct ScanLane {
         state = row * S;
         full = first + kChannels <= p.per_group;
     }
+    __device__ __forceinline__ bool exists(const ScanParams& p, int r, int s) const { return r < left && state + s < p.states; }
     // R neighbouring values of frame 4 i + row, or of frame `last` where that is behind it.  A whole block's are one
     // access without a branch; elsewhere the group's last channel stands in for those that do not exist.
     template <typename T>
@@ -287,6 +288,14 @@ __device__ __forceinline__ void scan_store_lanes(float* to, int64_t at, const Sc
         for (int k = 0; k < 4; ++k) v.v[k] = h[(q * 4 + k) / S][(q * 4 + k) % S];
         store_pack(base + q * 256, v);
     }
+}
+// Zeros in the place of what does not exist.
+template <int R, int S, bool Q>
+__device__ __forceinline__ void scan_clear_absent(const ScanParams& p, const ScanLane<R, S, Q>& w, float (&h)[R][S]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int s = 0; s < S; ++s) h[r][s] = w.exists(p, r, s) ? h[r][s] : 0.0f;
 }
 __device__ __forceinline__ int64_t scan_slot(const ScanUnit& u, int64_t t) {
     return u.begin / kScanSaveEvery + u.utt + (t - u.begin) / kScanSaveEvery;
@@ -539,6 +548,7 @@ __global__ __launch_bounds__(64 * kScanWaves, R < 4 && R * S <= 8 ? 4 : 1) void 
         if (MODE == 0) {
             if (p.state_out != nullptr && u.tail) scan_store_states(p.state_out, p, w, u.utt, h);
         } else {
+            scan_clear_absent(p, w, h);
             scan_store_lanes(p.seg_state, place, w, h);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
@@ -741,7 +751,8 @@ __device__ __forceinline__ void scan_sum_channels(const float (&b)[S], const flo
 // and the sum of its steps.  The states and decays of eight frames are held at once; with 64 states these are more
 // registers than two waves per SIMD have, and one wave with all of them takes half the time of two that spill (64
 // utterances of 100 to 300 frames x 1536 channels, forward and backward: 3.44 ms, now 1.69).
-template <typename T, int R, int S, bool GATE, int MODE>
+// PART: there are blocks with channels or states that do not exist (a branch over them costs whole blocks 1 %).
+template <typename T, int R, int S, bool GATE, int MODE, bool PART>
 __global__ __launch_bounds__(64 * kScanWaves, R * S > 8 ? 1 : 2) void scan_backward_kernel(ScanParams p) {
     constexpr int CH = 16 * R, NS = 4 * S, TILE = kScanSaveEvery;
     constexpr float kLn2 = 0.693147180559945309f;
@@ -938,6 +949,26 @@ __global__ __launch_bounds__(64 * kScanWaves, R * S > 8 ? 1 : 2) void scan_backw
                         }
                     if (k % 2 == 1) __builtin_amdgcn_sched_barrier(0);
                 }
+                if (PART && (!w.full || p.states != NS)) {
+                    // Channels and states that do not exist have the last channel's values, or zeros, and their states are
+                    // no one's concern until an infinity makes them NaN, which the sums below would take up.
+                    float odd = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int s = 0; s < S; ++s) odd = fmaf(h[TILE][r][s], 0.0f, odd);
+                    if (__any(odd != 0.0f)) {
+#pragma unroll
+                        for (int k = 0; k <= TILE; ++k)
+#pragma unroll
+                            for (int r = 0; r < R; ++r)
+#pragma unroll
+                                for (int s = 0; s < S; ++s) {
+                                    h[k][r][s] = w.exists(p, r, s) ? h[k][r][s] : 0.0f;
+                                    if (k < TILE) a[k][r][s] = w.exists(p, r, s) ? a[k][r][s] : 0.0f;
+                                }
+                    }
+                }
 #pragma unroll
                 for (int k = TILE - 1; k >= 0; --k) {
                     // A frame behind the utterance's last adds nothing to dA, but its zeros would, times an infinite
@@ -1051,6 +1082,7 @@ __global__ __launch_bounds__(64 * kScanWaves, R * S > 8 ? 1 : 2) void scan_backw
             if (MODE == 0) {
                 if (p.dstate_in != nullptr && u.head) scan_store_states(p.dstate_in, p, w, u.utt, g);
             } else {
+                scan_clear_absent(p, w, g);
                 scan_store_lanes(p.seg_state, place, w, g);
                 Pack<float, R> v;
 #pragma unroll
@@ -1235,17 +1267,19 @@ int scan_backward_launch(const ScanParams& q, hipStream_t st) {
     if (p.segment != 0) {
         const int64_t parts = p.parts;
         p.parts = p.units;
-        scan_backward_kernel<T, R, S, GATE, 1><<<scan_grid(p.units * across), 64 * kScanWaves, 0, st>>>(p);
+        scan_backward_kernel<T, R, S, GATE, 1, true><<<scan_grid(p.units * across), 64 * kScanWaves, 0, st>>>(p);
         SRX_HIP(hipGetLastError());
         scan_join_kernel<R, S, true><<<scan_grid(p.utts * p.blocks * (R * S / 4)), scan_join_threads(p), 0, st>>>(p);
         SRX_HIP(hipGetLastError());
         p.parts = parts;
     }
-    scan_backward_kernel<T, R, S, GATE, 0><<<scan_grid(p.parts * across), 64 * kScanWaves, 0, st>>>(p);
+    const unsigned wide = scan_grid(p.parts * across);
+    if (p.per_group % (16 * R) != 0 || p.states != 4 * S) scan_backward_kernel<T, R, S, GATE, 0, true><<<wide, 64 * kScanWaves, 0, st>>>(p);
+    else scan_backward_kernel<T, R, S, GATE, 0, false><<<wide, 64 * kScanWaves, 0, st>>>(p);
     SRX_HIP(hipGetLastError());
     const int64_t sums = p.utts > 0 ? p.frames * p.groups * 8 * S : 0;
-    const unsigned wide = sums > 0 ? scan_grid((sums + 255) / 256) : 0;
-    scan_sum_kernel<T, R, S><<<(unsigned)(p.blocks * (R * S / 4 + 1)) + wide, 256, 0, st>>>(p);
+    const unsigned more = sums > 0 ? scan_grid((sums + 255) / 256) : 0;
+    scan_sum_kernel<T, R, S><<<(unsigned)(p.blocks * (R * S / 4 + 1)) + more, 256, 0, st>>>(p);
     SRX_HIP(hipGetLastError());
     return SRX_OK;
 }

@@ -955,3 +955,16 @@ def test_scan_infinities_pass_from_piece_to_piece(sra, ctx, lengths, c, s, which
     rng = np.random.default_rng(38)
     off, t, v = _scan_case(rng, lengths, c, s, 1, "float32", state=False)
     _check_infinity(sra, ctx, off, t, v, "float32", rng, which)
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("which", ["x", "dt", "B"])
+@pytest.mark.parametrize("lengths,c,s,g", [([5, 9, 40], 20, 16, 1), ([21, 6], 70, 4, 1), ([24], 38, 8, 2), ([300], 20, 16, 1), ([19], 17, 64, 1)])
+def test_scan_infinities_meet_no_channels_that_do_not_exist(sra, ctx, lengths, c, s, g, which, dtype):
+    """The last channel stands in for those of a block that do not exist: an infinity of its own, or one of B, must not
+    reach the sums over the channels as NaN.  All signs alike, so that the definition adds up no infinities of both."""
+    torch = _torch()
+    rng = np.random.default_rng(s + c)
+    off, t, v = _scan_case(rng, lengths, c, s, g, dtype, state=False)
+    _check_infinity(sra, ctx, off, t, v, dtype, rng, which)
