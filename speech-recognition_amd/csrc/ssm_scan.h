@@ -575,9 +575,9 @@ __global__ __launch_bounds__(64 * kScanWaves, R < 4 && R * S <= 8 ? 4 : 1) void 
 // A state that is zero stays zero, and an infinite one infinite, as they do over the piece's frames one after the other:
 // the growth over all of a piece (an A above zero, or steps below) may be beyond 32 bits while that of every frame is not,
 // and its decay may be 0.
-__device__ __forceinline__ float scan_join(float log2_decay, float h, float own) {
+__device__ __forceinline__ float scan_join(float decay, float h, float own) {
     const bool scaled = h != 0.0f && fabsf(h) < __builtin_huge_valf();
-    return fmaf(scaled ? __builtin_amdgcn_exp2f(log2_decay) : 1.0f, h, own);
+    return fmaf(scaled ? decay : 1.0f, h, own);
 }
 constexpr int kJoinWaves = 16;
 inline int scan_join_threads(const ScanParams& p) { return 64 * (p.frames / (p.segment * p.utts) < 16 ? 4 : kJoinWaves); }
@@ -620,6 +620,12 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanParams p
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sum[a][e] = p.seg_sum[at * CH + w.col * R + (q * 4 + e) / S];
                 }
+                float by[AHEAD][4];
+#pragma unroll
+                for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) by[a][e] = __builtin_amdgcn_exp2f(sum[a][e] * A2[e]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int a = 0; a < AHEAD; ++a) {
                     if (k + a >= k1) break;
@@ -631,7 +637,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanParams p
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        h[e] = scan_join(sum[a][e] * A2[e], h[e], own[a].v[e]);
+                        h[e] = scan_join(by[a][e], h[e], own[a].v[e]);
                         decay[e] += sum[a][e];
                     }
                 }
@@ -648,7 +654,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanParams p
         for (int before = 0; before < wave; ++before)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                h[e] = scan_join(lds[before][1][w.lane][e] * A2[e], h[e], lds[before][0][w.lane][e]);
+                h[e] = scan_join(__builtin_amdgcn_exp2f(lds[before][1][w.lane][e] * A2[e]), h[e], lds[before][0][w.lane][e]);
         walk(true);
         __syncthreads();                                 // (the next task's results go to the same place)
     }
