@@ -968,3 +968,34 @@ def test_scan_infinities_meet_no_channels_that_do_not_exist(sra, ctx, lengths, c
     rng = np.random.default_rng(s + c)
     off, t, v = _scan_case(rng, lengths, c, s, g, dtype, state=False)
     _check_infinity(sra, ctx, off, t, v, dtype, rng, which)
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("which", ["x", "dt", "B"])
+@pytest.mark.parametrize("lengths,c,s,g", [([5, 9, 40], 20, 1, 1), ([21, 6], 70, 3, 1), ([5, 30], 40, 7, 2), ([17, 9], 33, 13, 1),
+                                           ([300], 20, 13, 1), ([300], 66, 2, 1), ([300], 40, 6, 2), ([300], 16, 20, 1),
+                                           ([9, 19], 17, 24, 1), ([11], 16, 33, 1), ([200], 18, 40, 1)])
+def test_scan_infinities_meet_no_states_that_do_not_exist(sra, ctx, lengths, c, s, g, which, dtype):
+    """A wave has room for 4, 8, 16, 32 or 64 states: those that there are not must not turn an infinite input into NaN."""
+    rng = np.random.default_rng(s + c)
+    off, t, v = _scan_case(rng, lengths, c, s, g, dtype, state=False)
+    _check_infinity(sra, ctx, off, t, v, dtype, rng, which)
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("s", [1, 2, 3, 7, 13, 16, 33])
+def test_scan_step_infinities_meet_no_states_that_do_not_exist(sra, ctx, s):
+    rng = np.random.default_rng(s)
+    off, t, v = _scan_case(rng, [1] * 4, 9, s, 1, "float32")
+    for k in ("x", "B", "C", "gate", "skip"):
+        t[k], v[k] = t[k].abs(), np.abs(v[k])
+    for q in (t, v):
+        q["x"][1, 3] = q["dt"][2, 4] = q["B"][3, 0, s - 1] = float("inf")
+    args = {q: v[q] for q in (*ORDER, *REST)}
+    ref, size = so.scan(off, **args), so.scan(off, scales=True, **args)
+    state = t["state"].clone()
+    y = sra.selective_scan_step(ctx, state, *(t[k] for k in ORDER), skip=t["skip"], gate=t["gate"], dt_bias=t["dt_bias"])
+    assert np.isinf(ref["y"][1, 3]) and np.isinf(ref["y"][2, 4]) and np.isinf(ref["y"][3]).all()
+    _same(y, ref["y"], size["y"], 4 + 2 * s + 40, "float32", "y")
+    _same(state, ref["state_out"], size["state_out"], 4 + 2 * s + 40, "float32", "state")
