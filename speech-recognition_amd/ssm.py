@@ -202,11 +202,10 @@ class _ScanCall:
                               _address(dt_bias))
         self.inputs = (x, dt, B, C_, gate)
         bc = groups * states
-        self.rows = _lib.ScanInputs(
-            x.data_ptr(), dt.data_ptr(), B.data_ptr(), C_.data_ptr(), _address(gate),
-            _rows(ctx, x, "x", rows, dtype, c), _rows(ctx, dt, "dt", rows, dtype, c),
-            _rows(ctx, B, "B", wide, dtype, bc), _rows(ctx, C_, "C", wide, dtype, bc),
-            0 if gate is None else _rows(ctx, gate, "gate", rows, dtype, c))
+        pitches = (_rows(ctx, x, "x", rows, dtype, c), _rows(ctx, dt, "dt", rows, dtype, c),
+                   _rows(ctx, B, "B", wide, dtype, bc), _rows(ctx, C_, "C", wide, dtype, bc),
+                   0 if gate is None else _rows(ctx, gate, "gate", rows, dtype, c))
+        self.rows = _lib.ScanInputs(x.data_ptr(), dt.data_ptr(), B.data_ptr(), C_.data_ptr(), _address(gate), *pitches)
 
     @staticmethod
     def _refuse(ctx, x, A, B):
@@ -412,6 +411,9 @@ def layer_norm_backward(ctx, dy, x, mean, rstd, weight=None):
     n, d = rows = tuple(x.shape)
     code, ld = _code(x, "x"), _rows(ctx, x, "x", rows, x.dtype, d)
     ld_dy = _rows(ctx, dy, "dy", rows, x.dtype, d)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t is None:
+            raise ValueError(f"{name} must be what layer_norm returned")
     mean, rstd = _parameter(ctx, mean, "mean", (n,)), _parameter(ctx, rstd, "rstd", (n,))
     weight = _parameter(ctx, weight, "weight", (d,))
     dx = _like(x)

@@ -281,3 +281,29 @@ def test_workspace_sizes_grow_with_the_problem():
     one = lib.srx_selective_scan_workspace(h, C.byref(scan), 1, 24000)                     # pieces of one
     assert one > 0 and lib.srx_selective_scan_backward_workspace(h, C.byref(scan), 1, 24000) > one
     assert lib.srx_selective_scan_saved(C.byref(scan), 1, 24000) == (3000 + 1) * 512 * 16
+
+
+@pytest.mark.parametrize("bad", [None, 1.0, [[0.0] * 4] * 6, np.zeros((6, 4), np.float32)])
+def test_what_is_no_tensor_is_refused_by_name(scan_args, bad):
+    import torch
+    import speech_recognition_amd as sra
+    a, x = scan_args, torch.zeros(6, 4)
+    for k in ("x", "dt", "A", "B", "C"):
+        _refused(f"{k} must be", sra.selective_scan, **{**a, k: bad})
+        _refused(f"{k} must be", sra.selective_scan_step, torch.zeros(6, 4, 3), **{**a, k: bad})
+        _refused(f"{k} must be", sra.selective_scan_backward, x, **{**a, k: bad})
+    _refused("dy must be", sra.selective_scan_backward, bad, **a)
+    _refused("dy must be", sra.causal_conv_backward, bad, x, torch.zeros(4, 3))
+    _refused("weight must be", sra.causal_conv, x, bad)
+    _refused("x must be", sra.causal_conv, bad, torch.zeros(4, 3))
+    _refused("x must be", sra.layer_norm, bad)
+    _refused("dy must be", sra.layer_norm_backward, bad, x, torch.zeros(6), torch.zeros(6))
+    _refused("mean must be", sra.layer_norm_backward, x, x, bad, torch.zeros(6))
+    _refused("rstd must be", sra.layer_norm_backward, x, x, torch.zeros(6), bad)
+    _refused(r"grads\[0\] must be", sra.clip_gradients, [bad], 1.0)
+    if bad is not None:
+        for k in ("gate", "skip", "dt_bias", "state"):
+            _refused(f"{k} must be", sra.selective_scan, **{**a, k: bad})
+        _refused("out must be", sra.selective_scan, out=bad, **a)
+        _refused("state_out must be", sra.selective_scan, state_out=bad, **a)
+        _refused("bias must be", sra.causal_conv, x, torch.zeros(4, 3), bias=bad)
