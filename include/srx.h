@@ -365,8 +365,10 @@ int srx_mstep(srx_handle_t h, const double* stats, const srx_priors_t* priors, i
  *     nothing is allocated, so the calls may be captured into graphs, and calls with
  *     workspaces of their own may run at the same time on several streams;
  *   - the caller's current device is left as it was;
- *   - frames before utt_offsets[0] and from utt_offsets[n_utts] on belong to no utterance: their
- *     rows in every output are left as they were. */
+ *   - frames before utt_offsets[0] and from utt_offsets[n_utts] on belong to no utterance: whatever they
+ *     hold has no part in anything, their gradients are 0, and their rows in y are left as they were, or set to
+ *     0 where SRX_ZERO_OTHER_ROWS is added to dtype (srx_causal_conv, srx_selective_scan). */
+enum { SRX_ZERO_OTHER_ROWS = 256 };
 
 /* Short causal convolution over the frames of each channel, one filter per channel:
  *   y[t, c] = act(bias[c] + sum_k weight[c, k] x[t - width + 1 + k, c])

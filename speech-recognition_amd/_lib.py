@@ -16,6 +16,7 @@ LIB_PATH = os.environ.get("SRX_LIB") or os.path.join(_HERE, "libsrx.so")
 
 SRX_F32, SRX_F64, SRX_BF16, SRX_F16 = 0, 1, 2, 3
 SRX_IDENTITY, SRX_SILU = 0, 1
+SRX_ZERO_OTHER_ROWS = 256
 SRX_MSTEP_FULL, SRX_MSTEP_TRANSITIONS_ONLY = 0, 1
 SRX_OPT_EXACT_F32 = 1
 SRX_OPT_ESTEP_PATH = 2

@@ -178,6 +178,20 @@ __device__ __forceinline__ float wave_sum(float v) {
     return halves_sum(v, v);
 }
 
+// Zeros in the rows of a matrix that belong to no utterance: those before off[0] and from off[utts] on (all, without
+// utterances).  Workgroup `group` of `groups` takes every groups-th of them.
+template <typename T>
+__device__ __forceinline__ void clear_other_rows(const int64_t* off, int64_t utts, int64_t frames, void* to, int64_t ld,
+                                                 int64_t width, int64_t group, int64_t groups) {
+    const int64_t first = utts > 0 ? min(max(off[0], (int64_t)0), frames) : 0;
+    const int64_t last = utts > 0 ? min(max(off[utts], first), frames) : 0;
+    for (int64_t i = group; i < frames - (last - first); i += groups) {
+        T* row = (T*)to + (i < first ? i : i + (last - first)) * ld;
+        for (int64_t c = threadIdx.x; c < width; c += blockDim.x) row[c] = (T)0.0f;
+    }
+}
+constexpr int kClearGroups = 64;        // workgroups behind a launch's own ones that do this: next to nothing if there is nothing to do
+
 // Parts [parts][columns] added up in a fixed order, 32 columns a workgroup and every 32nd part a thread; `store` takes
 // a column's sum.
 constexpr int kSumThreads = 1024;
@@ -227,6 +241,12 @@ struct DeviceGuard {
 };
 
 constexpr int kMostColumns = 1 << 24;           // values of a row, so that 32 bits count them and what lies beside them
+// Whether the caller wants zeros in y's rows of no utterance; leaves the element type.
+inline bool take_zero_rows(int& dtype) {
+    const bool zero = dtype >= 0 && (dtype & SRX_ZERO_OTHER_ROWS) != 0;
+    if (zero) dtype &= ~SRX_ZERO_OTHER_ROWS;
+    return zero;
+}
 inline bool frame_dtype(int dtype) { return dtype == SRX_F32 || dtype == SRX_BF16 || dtype == SRX_F16; }
 
 }  // namespace srx_frames

@@ -35,6 +35,7 @@ struct ConvParams {
     float* part;            // [parts, width + 1, channels]
     int64_t parts;
     float *dweight, *dbias;
+    int clear;              // workgroups (forward: rows of them) that set y's or dx's rows of no utterance to zero
 };
 
 struct ConvPiece {
@@ -100,12 +101,19 @@ __device__ __forceinline__ Pack<T, V> conv_row(const ConvParams& p, const ConvPi
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void conv_forward_kernel(ConvParams p, int64_t pieces) {
     const int c = (int)(blockIdx.x * blockDim.x + threadIdx.x) * V, left = p.channels - c;
+    const int groups = gridDim.y - p.clear;
+    if ((int)blockIdx.y >= groups) {
+        const int64_t group = (int64_t)(blockIdx.y - groups) * gridDim.x + blockIdx.x;
+        clear_other_rows<T>(p.off, p.utts, p.frames, p.y, p.ld_y, p.channels, group * blockDim.y + threadIdx.y,
+                            (int64_t)p.clear * gridDim.x * blockDim.y);
+        return;
+    }
     if (left <= 0) return;
     const bool all = (int)((blockIdx.x + 1) * blockDim.x) * V <= p.channels;      // (for the whole workgroup)
     ConvTaps<T, V, W> taps;
     taps.load(p, c, left);
     for (int64_t number = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; number < pieces;
-         number += (int64_t)gridDim.y * blockDim.y) {
+         number += (int64_t)groups * blockDim.y) {
         ConvPiece w;
         if (!conv_piece(p, number, w)) continue;
         Pack<T, V> row[W];                       // the frames under the filter, oldest first
@@ -298,7 +306,13 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvParams p, int64_
     }
 }
 
+template <typename T>
 __global__ __launch_bounds__(kSumThreads) void conv_sum_kernel(ConvParams p, int width) {
+    const int groups = gridDim.x - p.clear;
+    if ((int)blockIdx.x >= groups) {             // (the gradients of frames that belong to no utterance)
+        clear_other_rows<T>(p.off, p.utts, p.frames, p.dx, p.ld_dx, p.channels, blockIdx.x - groups, p.clear);
+        return;
+    }
     sum_parts(p.part, p.parts, (int64_t)(width + 1) * p.channels, [&](int64_t column, double s) {
         const int k = (int)(column / p.channels), c = (int)(column - (int64_t)k * p.channels);
         if (k < width) p.dweight[(int64_t)c * width + k] = (float)s;
@@ -316,6 +330,7 @@ int64_t conv_pieces(int64_t utts, int64_t frames) { return utts == 0 ? 0 : frame
 
 constexpr int kBackwardVector = 4;
 constexpr int kForwardVector = 4;
+constexpr int kClearRows = 16;          // of workgroups, for rows of no utterance
 
 int conv_lanes(int channels, int v) {
     const int vectors = (channels + v - 1) / v;
@@ -349,13 +364,13 @@ int conv_launch(const ConvParams& p, ConvWhat what, hipStream_t st) {
         const int lanes = conv_lanes(p.channels, FV), rows = 256 / lanes;
         const int64_t across = (p.channels + lanes * FV - 1) / (lanes * FV), groups = (pieces + rows - 1) / rows;
         const int64_t fill = (p.parts + across - 1) / across;       // (parts: the workgroups that the chip holds)
-        conv_forward_kernel<T, FV, W><<<dim3((unsigned)across, (unsigned)(groups < fill ? groups : fill)), dim3(lanes, rows), 0, st>>>(p, pieces);
+        conv_forward_kernel<T, FV, W><<<dim3((unsigned)across, (unsigned)(groups < fill ? groups : fill) + p.clear), dim3(lanes, rows), 0, st>>>(p, pieces);
     } else {
         const int lanes = conv_lanes(p.channels, kBackwardVector);
         const int across = (p.channels + lanes * kBackwardVector - 1) / (lanes * kBackwardVector);
         conv_backward_kernel<T, kBackwardVector, W><<<dim3((unsigned)across, (unsigned)p.parts), dim3(lanes, 256 / lanes), 0, st>>>(p, pieces);
         SRX_HIP(hipGetLastError());
-        conv_sum_kernel<<<((W + 1) * p.channels + 31) / 32, kSumThreads, 0, st>>>(p, W);
+        conv_sum_kernel<T><<<((W + 1) * p.channels + 31) / 32 + p.clear, kSumThreads, 0, st>>>(p, W);
     }
     SRX_HIP(hipGetLastError());
     return SRX_OK;
@@ -420,11 +435,12 @@ int srx_causal_conv(srx_handle_t h, const srx_conv_t* conv, int dtype, const voi
                     const int64_t* utt_offsets, int64_t n_utts, int64_t n_frames, const void* state_in,
                     void* state_out, void* y, int64_t ld_y, void* stream) {
     const char* who = "srx_causal_conv";
+    const bool zero = take_zero_rows(dtype) && n_frames > 0;
     int rc = check_conv(h, conv, n_utts, n_frames, who);
     if (rc) return rc;
     SRX_REQUIRE(frame_dtype(dtype), "%s: unknown dtype %d", who, dtype);
-    if (n_utts == 0) return SRX_OK;
-    SRX_REQUIRE(utt_offsets != nullptr, "%s: NULL utterance offsets", who);
+    if (n_utts == 0 && !zero) return SRX_OK;
+    SRX_REQUIRE(n_utts == 0 || utt_offsets != nullptr, "%s: NULL utterance offsets", who);
     SRX_REQUIRE(n_frames == 0 || (x != nullptr && y != nullptr), "%s: NULL x or y", who);
     SRX_REQUIRE(n_frames == 0 || (ld_x >= conv->n_channels && ld_y >= conv->n_channels),
                 "%s: a row pitch is smaller than its row", who);
@@ -434,6 +450,7 @@ int srx_causal_conv(srx_handle_t h, const srx_conv_t* conv, int dtype, const voi
     p.y = y;
     p.ld_y = ld_y;
     p.parts = (int64_t)h->n_cu * 16;
+    p.clear = zero ? kClearRows : 0;
     DeviceGuard guard(h->device);
     if (guard.rc) return guard.rc;
     return conv_run(p, conv->width, dtype, FORWARD, (hipStream_t)stream);
@@ -489,6 +506,7 @@ int srx_causal_conv_backward(srx_handle_t h, const srx_conv_t* conv, int dtype, 
     p.dstate_in = dstate_in;
     p.dweight = dweight;
     p.dbias = dbias;
+    p.clear = n_frames > 0 ? kClearGroups : 0;
     p.part = (float*)workspace;
     p.parts = conv_parts(h, conv->n_channels, n_utts, n_frames);
     DeviceGuard guard(h->device);

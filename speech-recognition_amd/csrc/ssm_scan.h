@@ -55,6 +55,7 @@ struct ScanParams {
     int round;               // utterances that give every CU a workgroup
     int* order;              // [utts] utterances by falling length, or NULL: as they come (the backward pass
                              // takes the forward pass's, behind the saved states)
+    int clear;               // workgroups that set the outputs' rows of no utterance to zero (0: these are left alone)
     // forward
     const float* state_in;   // [utts, channels, states] or NULL
     float* state_out;        // the same or NULL
@@ -413,7 +414,12 @@ __global__ __launch_bounds__(64 * kScanWaves, R < 4 && R * S <= 8 ? 4 : 1) void 
     float* sB = sU + TILE * CH;
     float* sC = sB + TILE * NS;
     const int across = (p.blocks + kScanWaves - 1) / kScanWaves;
-    for (int64_t task = blockIdx.x; task < p.units * across; task += gridDim.x) {
+    const int groups = gridDim.x - (MODE == 0 ? p.clear : 0);
+    if (MODE == 0 && (int)blockIdx.x >= groups) {
+        clear_other_rows<T>(p.off, p.utts, p.frames, p.y, p.ld_y, p.channels, blockIdx.x - groups, p.clear);
+        return;
+    }
+    for (int64_t task = blockIdx.x; task < p.units * across; task += groups) {
         const int64_t unit = task / across;
         const int block = (int)(task - unit * across) * kScanWaves + wave;
         ScanUnit u;
@@ -1232,12 +1238,24 @@ __device__ __forceinline__ void scan_sum_bc(const ScanParams& p, int64_t group, 
     }
 }
 
-// Both in one launch: the first workgroups take the parameters' parts, the others dB and dC.
+// All in one launch: the first workgroups take the parameters' parts, the last ones the gradients of the frames that belong
+// to no utterance, which are zero, the others dB and dC.
 template <typename T, int R, int S>
 __global__ __launch_bounds__(256) void scan_sum_kernel(ScanParams p) {
-    const unsigned parts = (unsigned)p.blocks * (R * S / 4 + 1);
-    if (blockIdx.x < parts) scan_sum_parts<R, S>(p, (int)blockIdx.x);
-    else scan_sum_bc<T, S>(p, blockIdx.x - parts, gridDim.x - parts);
+    const unsigned parts = (unsigned)p.blocks * (R * S / 4 + 1), clear = gridDim.x - p.clear;
+    if (blockIdx.x < parts) {
+        scan_sum_parts<R, S>(p, (int)blockIdx.x);
+    } else if (blockIdx.x < clear) {
+        scan_sum_bc<T, S>(p, blockIdx.x - parts, clear - parts);
+    } else {
+        void* const to[5] = {p.dx, p.ddt, p.dgate, p.dB, p.dC};
+        const int64_t ld[5] = {p.ld_dx, p.ld_ddt, p.ld_dgate, p.ld_dB, p.ld_dC};
+#pragma unroll
+        for (int k = 0; k < 5; ++k)
+            if (to[k] != nullptr)
+                clear_other_rows<T>(p.off, p.utts, p.frames, to[k], ld[k], k < 3 ? p.channels : p.groups * p.states,
+                                    blockIdx.x - clear, p.clear);
+    }
 }
 
 // ---- one frame of every stream --------------------------------------------------------------
@@ -1304,7 +1322,7 @@ int scan_forward_launch(const ScanParams& p, hipStream_t st) {
         scan_order_kernel<<<1, kScanOrdered, 0, st>>>(p);
         SRX_HIP(hipGetLastError());
     }
-    const unsigned wide = scan_grid(p.units * across);
+    const unsigned wide = scan_grid(p.units * across) + p.clear;
     if (p.states != 4 * S) scan_forward_kernel<T, R, S, GATE, 0, true><<<wide, 64 * kScanWaves, 0, st>>>(p);
     else scan_forward_kernel<T, R, S, GATE, 0, false><<<wide, 64 * kScanWaves, 0, st>>>(p);
     SRX_HIP(hipGetLastError());
@@ -1330,7 +1348,7 @@ int scan_backward_launch(const ScanParams& q, hipStream_t st) {
     SRX_HIP(hipGetLastError());
     const int64_t sums = p.utts > 0 ? p.frames * p.groups * 8 * S : 0;
     const unsigned more = sums > 0 ? scan_grid((sums + 255) / 256) : 0;
-    scan_sum_kernel<T, R, S><<<(unsigned)(p.blocks * (R * S / 4 + 1)) + more, 256, 0, st>>>(p);
+    scan_sum_kernel<T, R, S><<<(unsigned)(p.blocks * (R * S / 4 + 1)) + more + p.clear, 256, 0, st>>>(p);
     SRX_HIP(hipGetLastError());
     return SRX_OK;
 }

@@ -181,15 +181,17 @@ int srx_selective_scan(srx_handle_t h, const srx_scan_t* s, const srx_scan_input
                        float* state_out, void* y, int64_t ld_y, float* saved, void* workspace,
                        int64_t workspace_bytes, void* stream) {
     const char* who = "srx_selective_scan";
+    const bool zero = take_zero_rows(dtype) && n_frames > 0;
     int rc = check_scan(h, s, n_utts, n_frames, who);
     if (rc) return rc;
     if ((rc = check_inputs(s, in, dtype, n_frames, who))) return rc;
-    if (n_utts == 0) return SRX_OK;
-    SRX_REQUIRE(utt_offsets != nullptr, "%s: NULL utterance offsets", who);
+    if (n_utts == 0 && !zero) return SRX_OK;
+    SRX_REQUIRE(n_utts == 0 || utt_offsets != nullptr, "%s: NULL utterance offsets", who);
     SRX_REQUIRE(n_frames == 0 || y != nullptr, "%s: NULL y", who);
     SRX_REQUIRE(n_frames == 0 || (ld_y >= s->n_channels && pitch_fits(ld_y, s->n_channels, dtype, 4)),
                 "%s: a row pitch is smaller than its row, or 2^30 bytes or more", who);
     ScanParams p = params_for(h, s, n_utts, n_frames);
+    p.clear = zero ? kClearGroups : 0;
     p.saved = saved;
     if (saved != nullptr && p.ordered) p.order = (int*)(saved + saved_states(s, n_utts, n_frames));
     const int64_t need = carve(p, false, workspace);
@@ -243,7 +245,7 @@ int srx_selective_scan_backward(srx_handle_t h, const srx_scan_t* s, const srx_s
                 "%s: dskip / ddt_bias must be given exactly where skip / dt_bias are", who);
     SRX_REQUIRE(n_utts == 0 || utt_offsets != nullptr, "%s: NULL utterance offsets", who);
     if (n_frames > 0) {
-        SRX_REQUIRE(saved != nullptr && dy != nullptr, "%s: NULL saved or dy", who);
+        SRX_REQUIRE((saved != nullptr || n_utts == 0) && dy != nullptr, "%s: NULL saved or dy", who);
         SRX_REQUIRE(grads->dx && grads->ddt && grads->dB && grads->dC &&
                         (in->gate == nullptr) == (grads->dgate == nullptr),
                     "%s: NULL gradient of an input (dgate must be given exactly where gate is)", who);
@@ -255,6 +257,7 @@ int srx_selective_scan_backward(srx_handle_t h, const srx_scan_t* s, const srx_s
                     "%s: a row pitch of 2^30 bytes or more", who);
     }
     ScanParams p = params_for(h, s, n_utts, n_frames);
+    p.clear = n_frames > 0 ? kClearGroups : 0;
     p.saved = const_cast<float*>(saved);     // (the backward kernels only read it)
     if (p.ordered) p.order = (int*)(p.saved + saved_states(s, n_utts, n_frames));
     const int64_t need = carve(p, true, workspace);

@@ -10,8 +10,9 @@ Conventions of every function here:
   - frames are packed by utterance like ``Ragged.X``: (n_frames, channels), last dimension contiguous,
     rows at any pitch (a slice of a wider projection is taken as it is), float32, bfloat16 or float16;
   - ``offsets`` says where the utterances are: an int64 device tensor [U+1], a ``Ragged``, host
-    numbers, or None for one utterance.  Rows outside offsets[0] .. offsets[U] belong to none and stay
-    unwritten in every result;
+    numbers, or None for one utterance.  Rows outside offsets[0] .. offsets[U] belong to none: what they hold has
+    no part in anything, they stay as they are in an ``out`` that is given, and are 0 in results that the
+    functions make themselves and in gradients;
   - parameters, scan states and parameters' gradients are float32 whatever the frames are; arithmetic
     is in 32 bits, a result is rounded once;
   - work is queued on the current torch stream of the context's device.  Nothing is kept between calls
@@ -246,7 +247,8 @@ def selective_scan(ctx, x, dt, A, B, C, offsets=None, skip=None, gate=None, dt_b
     if save:
         saved = torch.empty((lib.srx_selective_scan_saved(_ref(a.scan), utts, a.n),), dtype=torch.float32,
                             device=ctx.device)
-    check(lib.srx_selective_scan(ctx.handle, _ref(a.scan), _ref(a.rows), a.code, off.data_ptr(), utts, a.n,
+    code = a.code if out is not None else a.code | _lib.SRX_ZERO_OTHER_ROWS
+    check(lib.srx_selective_scan(ctx.handle, _ref(a.scan), _ref(a.rows), code, off.data_ptr(), utts, a.n,
                                  _address(state), state_out.data_ptr(), y.data_ptr(), ld_y,
                                  _address(saved), _address(ws), 0 if ws is None else ws.numel(),
                                  ctx.stream_ptr()), "srx_selective_scan")
@@ -344,7 +346,8 @@ def causal_conv(ctx, x, weight, offsets=None, bias=None, activation=None, state=
     else:
         _state(ctx, state_out, "state_out", shape, x.dtype)
         _apart(state_out, "state_out", x, *a.keep, y, None if state_out is state else state)
-    check(lib.srx_causal_conv(ctx.handle, _ref(a.conv), a.code, x.data_ptr(), a.ld, off.data_ptr(), utts, a.n,
+    code = a.code if out is not None else a.code | _lib.SRX_ZERO_OTHER_ROWS
+    check(lib.srx_causal_conv(ctx.handle, _ref(a.conv), code, x.data_ptr(), a.ld, off.data_ptr(), utts, a.n,
                               _address(state), state_out.data_ptr(), y.data_ptr(), ld_y,
                               ctx.stream_ptr()), "srx_causal_conv")
     return y, state_out

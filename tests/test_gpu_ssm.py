@@ -999,3 +999,56 @@ def test_scan_step_infinities_meet_no_states_that_do_not_exist(sra, ctx, s):
     assert np.isinf(ref["y"][1, 3]) and np.isinf(ref["y"][2, 4]) and np.isinf(ref["y"][3]).all()
     _same(y, ref["y"], size["y"], 4 + 2 * s + 40, "float32", "y")
     _same(state, ref["state_out"], size["state_out"], 4 + 2 * s + 40, "float32", "state")
+
+
+# ---- rows that belong to no utterance ------------------------------------------------------------------------------------
+
+def _dirty(*shapes):
+    """Leaves memory of these sizes full of NaN behind with torch's allocator."""
+    torch = _torch()
+    for _ in range(3):
+        held = [torch.full(s, float("nan"), dtype=d, device="cuda") for s, d in shapes for _ in range(8)]
+        del held
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("lengths,lead,tail,c,s,g", [([12, 0, 21], 3, 4, 37, 7, 1), ([700], 5, 1, 24, 16, 1), ([], 3, 4, 20, 16, 2),
+                                                     ([3], 900, 1000, 40, 24, 1), (list(range(20, 60)), 1, 2, 1650, 16, 1)])
+def test_results_that_are_new_are_zero_in_rows_of_no_utterance(sra, ctx, lengths, lead, tail, c, s, g, dtype):
+    """Frames outside every utterance take no part: their gradients are 0, and so are their rows in results that the
+    functions themselves allocate, whatever they hold as inputs; where the offsets come from does not matter."""
+    torch = _torch()
+    rng = np.random.default_rng(34)
+    off, t, v = _scan_case(rng, lengths, c, s, g, dtype, state=False)
+    inside, n = int(off[-1]), int(off[-1]) + lead + tail
+
+    def room(a):
+        wide = torch.full((n, *a.shape[1:]), float("nan"), dtype=a.dtype, device="cuda")
+        wide[lead:lead + inside] = a
+        return wide
+
+    wide = {k: room(t[k]) for k in ("x", "dt", "B", "C", "gate")}
+    dy = _draw(rng, (inside, c), dtype)[0]
+    w = torch.from_numpy(rng.standard_normal((c, 4)).astype(np.float32)).cuda()
+    want = _run_scan(sra, ctx, off, t, dy)
+    grad = sra.causal_conv_backward(ctx, dy, t["x"], w, torch.from_numpy(off).cuda(), None, "silu")
+    plain = sra.causal_conv(ctx, t["x"], w, torch.from_numpy(off).cuda(), None, "silu")[0]
+    for offsets in (torch.from_numpy(off + lead).cuda(), off + lead):
+        o = dict(offsets=offsets)
+        _dirty(((n, c), t["x"].dtype), ((n, g, s), t["x"].dtype))
+        rest, args = {k: {**t, **wide}[k] for k in REST}, [{**t, **wide}[k] for k in ORDER]
+        y, last, saved = sra.selective_scan(ctx, *args, save=True, **o, **rest)
+        _dirty(((n, c), t["x"].dtype), ((n, g, s), t["x"].dtype))
+        got = sra.selective_scan_backward(ctx, room(dy), *args, saved=saved, **o, **rest)
+        pairs = [("y", y, want[0]), *((k, got[k], want[2][k]) for k in ("x", "dt", "B", "C", "gate"))]
+        _dirty(((n, c), t["x"].dtype))
+        pairs.append(("conv", sra.causal_conv(ctx, wide["x"], w, activation="silu", **o)[0], plain))
+        _dirty(((n, c), t["x"].dtype))
+        back = sra.causal_conv_backward(ctx, room(dy), wide["x"], w, activation="silu", **o)
+        pairs.append(("conv dx", back["x"], grad["x"]))
+        for k, a, b in pairs:
+            assert torch.equal(a[lead:lead + inside], b), k
+            assert not a[:lead].any() and not a[lead + inside:].any(), k
+        assert torch.equal(last, want[1])
+        for a in (got["A"], got["skip"], got["dt_bias"], back["weight"]):        # (their sums' order may differ)
+            assert torch.isfinite(a).all()
