@@ -16,8 +16,8 @@ Conventions of every function here:
   - parameters, scan states and parameters' gradients are float32 whatever the frames are; arithmetic
     is in 32 bits, a result is rounded once;
   - work is queued on the current torch stream of the context's device.  Nothing is kept between calls
-    and scratch comes from torch's allocator, so calls may be captured into graphs and run on several
-    streams of one context;
+    and scratch comes from torch's allocator, so calls may be captured into graphs (but for those with host
+    numbers as offsets, which copy them) and run on several streams of one context;
   - gradients are explicit: the ``*_backward`` functions are called with the gradient of the result,
     torch's autograd is not involved (a tensor that requires grad is refused while it records).
 """
@@ -114,8 +114,13 @@ def _offsets(ctx, offsets, n_frames):
         if offsets.dim() != 1 or offsets.numel() < 1 or offsets.dtype != torch.int64 or offsets.device != ctx.device:
             raise ValueError(f"offsets must be an int64 tensor [U+1] on {ctx.device}")
         return offsets.contiguous()
-    if offsets is None:
-        return ctx.tensor(np.array([0, n_frames], dtype=np.int64))
+    if offsets is None:                             # (made on the device: nothing is copied or waited for)
+        kind = dict(dtype=torch.int64, device=ctx.device)
+        return torch.arange(0, 2 * n_frames, n_frames, **kind) if n_frames else torch.zeros(2, **kind)
+    if ctx.device.type == "cuda":
+        with torch.cuda.device(ctx.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("offsets in host memory would be copied while a graph is captured: give a device tensor")
     off = np.asarray(offsets, dtype=np.int64).reshape(-1)
     if off.size < 1 or off[0] < 0 or off[-1] > n_frames:
         raise ValueError(f"offsets must lie between 0 and {n_frames}")

@@ -1052,3 +1052,37 @@ def test_results_that_are_new_are_zero_in_rows_of_no_utterance(sra, ctx, lengths
         assert torch.equal(last, want[1])
         for a in (got["A"], got["skip"], got["dt_bias"], back["weight"]):        # (their sums' order may differ)
             assert torch.isfinite(a).all()
+
+
+# ---- captured calls without offsets --------------------------------------------------------------------------------------
+
+def test_captured_without_offsets(sra, ctx):
+    """None is one utterance, made on the device; host numbers would be copied while a graph is captured and are refused
+    before anything is recorded."""
+    torch = _torch()
+    rng = np.random.default_rng(37)
+    off, t, v = _scan_case(rng, [50], 24, 16, 1, "float32")
+    w = torch.from_numpy(rng.standard_normal((24, 4)).astype(np.float32)).cuda()
+    dy = _draw(rng, (50, 24), "float32")[0]
+
+    def step():
+        u, _ = sra.causal_conv(ctx, t["x"], w, activation="silu")
+        args, rest = (u, t["dt"], t["A"], t["B"], t["C"]), {k: t[k] for k in REST}
+        y, last, saved = sra.selective_scan(ctx, *args, save=True, **rest)
+        g = sra.selective_scan_backward(ctx, dy, *args, saved=saved, **rest)
+        return [y, last, *g.values(), sra.causal_conv_backward(ctx, g["x"], t["x"], w, activation="silu")["weight"]]
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        with pytest.raises(ValueError, match="captured"):
+            sra.causal_conv(ctx, t["x"], w, [0, 50])
+        held = step()
+    for rep in range(4):
+        t["x"].copy_(torch.from_numpy(rng.standard_normal((50, 24)).astype(np.float32)))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for a, b in zip(held, want):
+            assert torch.equal(a, b), rep
