@@ -339,13 +339,16 @@ int conv_lanes(int channels, int v) {
     return lanes;
 }
 // Workgroups along the pieces: enough to fill the chip several times over, and few enough frames per thread
-// (512 at most) that the 32-bit sums of the taps' gradients stay exact to a few units of rounding.
+// that the 32-bit sums of the taps' gradients stay exact to a few units of rounding.  (Beyond what a grid's second
+// dimension has room for, 130 million frames at the least, the sums get longer.)
+constexpr int kConvMostSummed = 512;
 int64_t conv_parts(const srx_context* h, int channels, int64_t utts, int64_t frames) {
     const int lanes = conv_lanes(channels, kBackwardVector), rows = 256 / lanes;
     const int64_t across = (channels + lanes * kBackwardVector - 1) / (lanes * kBackwardVector);
     const int64_t groups = (conv_pieces(utts, frames) + rows - 1) / rows;
     const int64_t fill = ((int64_t)h->n_cu * 8 + across - 1) / across;
-    const int64_t exact = (groups + 31) / 32;
+    constexpr int64_t most = kConvMostSummed / kConvPiece;
+    const int64_t exact = (groups + most - 1) / most;
     const int64_t parts = groups < fill ? groups : fill > exact ? fill : exact;
     return parts < 1 ? 1 : parts < 65535 ? parts : 65535;              // (a grid's second dimension)
 }

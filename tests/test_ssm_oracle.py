@@ -307,3 +307,16 @@ def test_what_is_no_tensor_is_refused_by_name(scan_args, bad):
         _refused("out must be", sra.selective_scan, out=bad, **a)
         _refused("state_out must be", sra.selective_scan, state_out=bad, **a)
         _refused("bias must be", sra.causal_conv, x, torch.zeros(4, 3), bias=bad)
+
+
+def test_conv_backward_sums_at_most_512_frames_in_a_row():
+    """The taps' gradients: every thread's own sum in 32 bits, the rest in 64.  16 pieces of 32 frames a thread, as long
+    as a grid's second dimension has room."""
+    from speech_recognition_amd import _lib
+    h = _Stub().handle
+    for channels, lanes in ((256, 64), (32, 8), (1000, 64)):
+        for utts, frames in ((1, 100), (64, 12800), (1, 1 << 20), (5000, 10 ** 7), (1, 10 ** 8)):
+            size = _lib.lib.srx_causal_conv_backward_workspace(h, C.byref(_lib.Conv(channels, 4, 0, 0, 1, None)), utts, frames)
+            parts, rows = size // (5 * channels * 4), 256 // lanes
+            pieces = frames // 32 + utts
+            assert -(-pieces // (parts * rows)) * 32 <= 512, (channels, utts, frames, parts)
