@@ -7,6 +7,9 @@ namespace {
 // States of a wave: 4 S.
 int block_states(int states) { return states <= 4 ? 4 : states <= 8 ? 8 : states <= 16 ? 16 : states <= 32 ? 32 : 64; }
 
+// Channels of a lane, at most (params_for takes one where two leave too few waves).
+int most_wide(int states) { return states <= 4 ? 4 : states <= 16 ? 2 : 1; }
+
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 int check_scan(srx_handle_t h, const srx_scan_t* s, int64_t utts, int64_t frames, const char* who) {
@@ -60,8 +63,8 @@ ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, i
     // Two channels a lane, or one where two leave too few waves (the work beside the exponentials is smaller for
     // two) and from 17 states on, whose registers leave no room for more.  Utterances of 200 frames x 1024 channels, 16
     // states, forward and backward: 32 of them 173 us with two and 158 with one, 64 of them 261 and 300.
-    p.wide = s->n_states <= 4 ? 4 : 2;
-    if (s->n_states > 16 || (s->n_states > 8 && utts * blocks_of(2) < 2 * simds)) p.wide = 1;
+    p.wide = most_wide(s->n_states);
+    if (s->n_states > 8 && utts * blocks_of(2) < 2 * simds) p.wide = 1;
     p.group_blocks = (p.per_group + 16 * p.wide - 1) / (16 * p.wide);
     p.blocks = p.group_blocks * s->n_groups;
     // Whole utterances where they alone give every SIMD a wave; else pieces, whose states are computed twice: shorter ones
@@ -93,7 +96,7 @@ ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, i
 }
 
 int64_t saved_states(const srx_scan_t* s, int64_t utts, int64_t frames) {
-    const int64_t ch = 64, per = s->n_channels / s->n_groups;      // (room for every way to cut the channels)
+    const int64_t ch = 16 * most_wide(s->n_states), per = s->n_channels / s->n_groups;      // (room for every way to cut the channels)
     return (frames / kScanSaveEvery + utts) * ((per + ch - 1) / ch * s->n_groups) * ch * block_states(s->n_states);
 }
 

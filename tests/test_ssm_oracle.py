@@ -320,3 +320,14 @@ def test_conv_backward_sums_at_most_512_frames_in_a_row():
             parts, rows = size // (5 * channels * 4), 256 // lanes
             pieces = frames // 32 + utts
             assert -(-pieces // (parts * rows)) * 32 <= 512, (channels, utts, frames, parts)
+
+
+@pytest.mark.parametrize("channels,states,groups", [(20, 16, 5), (40, 12, 40), (512, 17, 1), (100, 64, 1), (66, 3, 2), (70, 8, 1)])
+def test_saved_states_take_room_for_the_widest_block_and_no_more(channels, states, groups):
+    """Channels of a group up to whole blocks of 64 (up to 4 states), 32 (up to 16) or 16, states up to 4, 8, 16, 32 or 64."""
+    from speech_recognition_amd import _lib
+    block, room = (64 if states <= 4 else 32 if states <= 16 else 16), next(r for r in (4, 8, 16, 32, 64) if states <= r)
+    for utts, frames in ((1, 1000), (3, 50), (40, 5000)):
+        size = _lib.lib.srx_selective_scan_saved(C.byref(_lib.Scan(channels, states, groups, 1, 1, None, None)), utts, frames)
+        wide = -(-(channels // groups) // block) * block * groups
+        assert size == (frames // 8 + utts) * wide * room + (utts if utts >= 16 else 0)
