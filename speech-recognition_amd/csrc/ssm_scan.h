@@ -1309,10 +1309,13 @@ inline unsigned scan_grid(int64_t tasks) {
     return (unsigned)(tasks < 1 ? 1 : tasks < kScanMostWorkgroups ? tasks : kScanMostWorkgroups);
 }
 
+// Whether utterances are ever cut into pieces: two channels a lane with 16 states are for batches that fill the device.
+constexpr bool scan_cuts(int R, int S) { return !(R == 2 && S == 4); }
+
 template <typename T, int R, int S, bool GATE>
 int scan_forward_launch(const ScanParams& p, hipStream_t st) {
     const int64_t across = (p.blocks + kScanWaves - 1) / kScanWaves;
-    if (p.segment != 0) {
+    if constexpr (scan_cuts(R, S)) if (p.segment != 0) {
         scan_forward_kernel<T, R, S, GATE, 1, false><<<scan_grid(p.units * across), 64 * kScanWaves, 0, st>>>(p);
         SRX_HIP(hipGetLastError());
         scan_join_kernel<R, S, false><<<scan_grid(p.utts * p.blocks * (R * S / 4)), scan_join_threads(p), 0, st>>>(p);
@@ -1333,7 +1336,7 @@ template <typename T, int R, int S, bool GATE>
 int scan_backward_launch(const ScanParams& q, hipStream_t st) {
     ScanParams p = q;
     const int64_t across = (p.blocks + kScanWaves - 1) / kScanWaves;
-    if (p.segment != 0) {
+    if constexpr (scan_cuts(R, S)) if (p.segment != 0) {
         const int64_t parts = p.parts;
         p.parts = p.units;
         scan_backward_kernel<T, R, S, GATE, 1, true><<<scan_grid(p.units * across), 64 * kScanWaves, 0, st>>>(p);

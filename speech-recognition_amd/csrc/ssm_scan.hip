@@ -73,7 +73,7 @@ ScanParams params_for(const srx_context* h, const srx_scan_t* s, int64_t utts, i
     // frames whole 19 us (67), in pieces 24 (69); 300 frames 43 (158) and 24 (69), in pieces of 64 28 (81).
     p.segment = 0;
     p.units = utts;
-    if (utts > 0 && utts * p.blocks < simds) {
+    if (utts > 0 && utts * p.blocks < simds) {           // (so never with two channels a lane and 16 states)
         const int64_t even = frames * p.blocks / (4 * simds), least = frames * p.blocks < 64 * simds ? 32 : 64;
         const int64_t segment = round_up(even > least ? even : least, 16);
         if ((utts == 1 ? frames : 2 * (frames / utts)) > 7 * segment / 2) {
