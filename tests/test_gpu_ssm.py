@@ -1086,3 +1086,26 @@ def test_captured_without_offsets(sra, ctx):
         torch.cuda.synchronize()
         for a, b in zip(held, want):
             assert torch.equal(a, b), rep
+
+
+# ---- shapes of the pieces, of utterances by length, and of whole blocks --------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("lengths,c,s,g", [([700], 130, 4, 1), ([300, 41], 66, 3, 1), ([700], 40, 8, 1), ([129, 300], 96, 5, 2),
+                                           ([700], 33, 24, 1), ([300, 0, 129], 40, 32, 2), ([500], 17, 64, 1)])
+def test_scan_pieces_of_every_number_of_states(sra, ctx, lengths, c, s, g, dtype):
+    rng = np.random.default_rng(35)
+    off, t, v = _scan_case(rng, lengths, c, s, g, dtype)
+    _check_scan(sra, ctx, off, t, v, dtype, rng)
+
+
+@pytest.mark.parametrize("dtype,lengths,c,s,g", [("float32", 40, 3328, 4, 1), ("bfloat16", 40, 3300, 3, 2), ("float16", 40, 1650, 16, 1),
+                                                 ("float16", 40, 832, 24, 1), ("bfloat16", 40, 840, 64, 1),
+                                                 ("float32", 1100, 65, 12, 1)])
+def test_scan_more_batches_that_fill_the_device(sra, ctx, dtype, lengths, c, s, g):
+    """Utterances by length for the other numbers of states, and more utterances than are put in order."""
+    rng = np.random.default_rng(36)
+    lengths = rng.integers(25, 50, lengths) if lengths < 100 else rng.integers(0, 9, lengths)
+    lengths[5], lengths[8] = 0, 60
+    off, t, v = _scan_case(rng, lengths, c, s, g, dtype)
+    _check_scan(sra, ctx, off, t, v, dtype, rng)
