@@ -432,8 +432,9 @@ typedef struct {
     void *dx, *ddt, *dB, *dC, *dgate;
     int64_t ld_dx, ld_ddt, ld_dB, ld_dC, ld_dgate;
 } srx_scan_gradients_t;
-/* Floats of `saved`: what a training pass keeps for srx_selective_scan_backward (every eighth frame's states, and the
- * order in which a full device takes the utterances). */
+/* Floats of `saved`: what a training pass keeps for srx_selective_scan_backward (the states before every eighth frame, a row
+ * more per utterance, states and channels rounded up to whole blocks; and the order in which a full device takes the
+ * utterances). */
 int64_t srx_selective_scan_saved(const srx_scan_t* scan, int64_t n_utts, int64_t n_frames);
 int64_t srx_selective_scan_workspace(srx_handle_t h, const srx_scan_t* scan, int64_t n_utts, int64_t n_frames);
 /* saved: NULL, or srx_selective_scan_saved floats to fill. */

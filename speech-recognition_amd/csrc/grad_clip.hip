@@ -3,7 +3,7 @@
 // same order (no value travels through the host, no atomics, the same bits every time) and multiplies.
 // The tensors' addresses travel in the kernels' arguments, kTensors per launch, so that nothing is
 // uploaded and the calls can be captured; every workgroup takes them into LDS in one go and searches there.
-// 157 million bfloat16 values into float32: 296 us.  The first pass reads 3.0 TB/s (behind the writes of the call
+// 157 million bfloat16 values into float32: 296 us.  The first pass reads 3.2 TB/s (behind the writes of the call
 // before), the second reads and writes 4.4 TB/s, part of its reads from the memory-side cache, which is why it runs
 // backwards, in a launch and over the launches (315 us without the latter).  Stores that pass by the caches: 309 us.
 #include "frame_ops.h"

@@ -2,7 +2,9 @@
 // A row is held in registers by 16 or 64 lanes of a wave or by a whole workgroup, by its width, and read
 // once: mean first, then the squares of what is left, so that a mean far from zero costs no accuracy.
 // Wider rows than a workgroup's registers hold are read again for each of the passes.  65,536 rows of 1024 values in
-// bfloat16: forward 54 us, backward 80 us, both 5.0 TB/s; 1,310,720 rows of 39 in float32: 84 us, 4.9 TB/s.
+// bfloat16: forward 55 us, backward 83 us, 4.9 TB/s; 1,310,720 rows of 39 in float32: 85 us, 4.8 TB/s.
+// Slower: the backward pass of narrow rows (1,310,720 of 39: 153 us, 4.0 TB/s, in bfloat16 159 us, 1.9), and rows above 4096
+// (6000 of 8192 in float32: 148 and 419 us, 2.7 and 1.4 TB/s).
 #include "frame_ops.h"
 
 using namespace srx_frames;

@@ -19,9 +19,9 @@
 //
 // Bound by the vector ALU: per (frame, channel, state) an exponential, two products and two multiply-adds, 9 ns of a
 // SIMD per 64 of them, and about two thirds of that again for what a frame needs per channel and for LDS.  A recording
-// of 24,001 frames x 512 channels x 16 states in bfloat16 takes 112 us (28 for the recursion's arithmetic alone, 20 for
+// of 24,001 frames x 512 channels x 16 states in bfloat16 takes 113 us (28 for the recursion's arithmetic alone, 20 for
 // its bytes; cut into pieces it is computed twice), 96 utterances of 100 to 300 frames x 1024 channels in float16
-// 102 us (44, 35), forward and backward over 64 such x 1536 channels in bfloat16 401 us (124, 66).  One channel per lane
+// 104 us (44, 35), forward and backward over 64 such x 1536 channels in bfloat16 402 us (124, 66).  One channel per lane
 // with all its states, which needs no sums across lanes and no LDS but for B and C, has 8 % fewer instructions but
 // registers for two waves per SIMD only, and is slower (124, 142).
 #pragma once
@@ -717,6 +717,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanParams p
 // channels, here neighbours (two quad permutations per sum); sums over the channels (dB, dC) cross the 16 lanes that
 // share states: the first two of their four steps exchange whole halves and rows between two
 // registers, so that each step halves the number of registers too.
+//
+// What does not exist (channels and states of a block, frames behind the last) has zeros for all that is its own, which an
+// infinite state or input of those that there are would turn into NaN; it is kept from that.  An infinite gradient is not kept
+// from it, nor an infinite C: sums that the definition makes infinite may be NaN then, finite ones stay.
 
 template <typename T, int R, int S, bool GATE>
 struct ScanOctetRaw {

@@ -234,7 +234,7 @@ def selective_scan(ctx, x, dt, A, B, C, offsets=None, skip=None, gate=None, dt_b
     skip, dt_bias: (channels,).  state: (U, channels, states) float32, the states before the first
     frames (zeros without it); state_out, which may be ``state`` itself, receives those behind the last
     frames (unchanged for an utterance without frames), so that a recording can come in pieces.  Up to 64
-    states.  Returns (y, state_out), with save=True (y, state_out, saved): saved is what
+    states.  An A of minus infinity forgets at once; a step of 0 leaves a state as it is, whatever A is.  Returns (y, state_out), with save=True (y, state_out, saved): saved is what
     ``selective_scan_backward`` wants of this pass."""
     a = _ScanCall(ctx, x, dt, A, B, C, skip, gate, dt_bias, dt_softplus)
     off = _offsets(ctx, offsets, a.n)
